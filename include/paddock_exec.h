@@ -43,7 +43,8 @@ enum PdxPlaneKind {
     PDX_PLANE_KQ = 2,     /* RepackedKQ: k-quant data + 24-byte records */
     PDX_PLANE_F8ROW = 3,  /* F8RowPlane: e4m3 [out][in] + one f32 scale per row */
     PDX_PLANE_NVF4 = 4,   /* Nvf4Plane: e2m1 pairs [out][in/2] + e4m3 [out][in/16] + scale2 */
-    PDX_PLANE_MXFP4 = 5   /* RepackedMxfp4: 16 data bytes + 1 e8m0 byte per block, split */
+    PDX_PLANE_MXFP4 = 5,  /* RepackedMxfp4: 16 data bytes + 1 e8m0 byte per block, split */
+    PDX_PLANE_F8BLK = 6   /* e4m3 [out][in] + one f32 scale per 128 x 128 tile (no counterpart in the reference) */
 };
 /* gpu/types.rs:146-160; this pack reads the Row order only */
 enum PdxNvf4Layout { PDX_NVF4_ROW = 0, PDX_NVF4_TILED = 1, PDX_NVF4_FRAG = 2 };
@@ -113,6 +114,10 @@ int pdx_bf16_to_f8row(PdxExecutor* ex, const void* bf16, uint64_t in_dim, uint64
 /* an FP8 per-channel checkpoint (pdk_st_fp8_channel_view) uploaded as it is */
 int pdx_f8row_upload(PdxExecutor* ex, const void* e4m3, const float* row_scales, uint64_t in_dim, uint64_t out_dim,
                      PdxPlane** out);
+/* block-scaled e4m3: host bf16 [out][in] quantized on the device, or a checkpoint's codes and scales
+ * (f32 [ceil(out/128)][ceil(in/128)]) uploaded as they are.  in_dim a multiple of 16. */
+int pdx_bf16_to_f8blk(PdxExecutor* ex, const void* bf16, uint64_t in_dim, uint64_t out_dim, PdxPlane** out);
+int pdx_f8blk_upload(PdxExecutor* ex, const void* e4m3, const float* scales, uint64_t in_dim, uint64_t out_dim, PdxPlane** out);
 /* nvf4_upload (gpu/fp4.rs:1125-1168): the checkpoint triple byte for byte, sizes checked against
  * the dims, plus nvf4_tc5_tile (fp4.rs:1712-1746) when in_dim is whole 256-element slabs */
 int pdx_nvf4_upload(PdxExecutor* ex, const void* packed, uint64_t packed_len, const void* scales, uint64_t scales_len,
@@ -138,6 +143,15 @@ int pdx_rmsnorm_quant_e4m3_row(PdxExecutor* ex, const void* x, const void* w, vo
                                float eps, uint32_t batch, int* fused);
 int pdx_add_rmsnorm_scaled_quant_e4m3_row(PdxExecutor* ex, void* x, const void* proj, const void* w, void* xn, void* q,
                                           void* rs, uint32_t n, float eps, float pscale, uint32_t batch, int* fused);
+/* block-scaled e4m3 (paddock_pack.h has the formats): the activation quantizer, its form behind residual add and RMSNorm (proj and
+ * xn may be NULL), the product (y f32) and the gated front of a feed-forward block.  PDX_MISSING_OP on a pack without them. */
+int pdx_quantize_e4m3_blk(PdxExecutor* ex, const void* x, void* q, void* scale, uint32_t n, uint32_t batch);
+int pdx_add_rmsnorm_quant_e4m3_blk(PdxExecutor* ex, void* x, const void* proj, const void* w, void* xn, void* q, void* scale,
+                                   uint32_t n, float eps, uint32_t batch);
+int pdx_f8blk_dequant(PdxExecutor* ex, const PdxPlane* w, void* out_f32);
+int pdx_f8blk_gemm(PdxExecutor* ex, const PdxPlane* w, const void* xq, const void* xs, void* y, uint32_t batch);
+int pdx_f8blk_gate_up(PdxExecutor* ex, const PdxPlane* gate, const PdxPlane* up, const void* xq, const void* xs, void* hq, void* hs,
+                      uint32_t batch);
 /* quantize_nvf4 (gpu/fp4.rs:181-205), nvf4_gemm_f4 (fp4.rs:1902-1975: Row layout only; the tcgen05
  * slot when the plane carries tiled scales) and the W4A16 decode GEMV (slot nvf4_gemv) */
 int pdx_quantize_nvf4(PdxExecutor* ex, const void* x, void* q, void* scale, uint32_t n);

@@ -222,6 +222,36 @@ int pdk_f8row_gemm_bf16(const void* data, const void* w_rowscale, const void* xq
  * device, so it is a test / diagnostics call, never part of a launch path. */
 unsigned int pdk_device_error(void);
 
+/* ---- FP8 E4M3, one f32 scale per block of 128 ---------------------------------
+ * No slots: the reference has no block-scaled e4m3 format.  The one of FP8 checkpoints that carry `weight_scale_inv`:
+ *   weights      data e4m3 [out][in], scale f32 [ceil(out/128)][ceil(in/128)], one per 128 x 128 tile; w = code * scale.
+ *                A checkpoint's two tensors are these planes byte for byte.
+ *   activations  q e4m3 [batch][in], scale f32 [batch][ceil(in/128)], one per token and 128 elements.
+ * Quantizer of a block: a = max |v|, scale = max(a / 448, 2^-126), code = RN_e4m3(v * (1 / scale)), saturating, in f32.  A NaN or an
+ * infinity makes every product of its token NaN. */
+
+/* activations f32 / bf16 [batch][n] -> q, scale.  Any n; rows of whole 16-byte pieces on 16-byte boundaries are the fast case. */
+int pdk_quantize_e4m3_blk(const void* x, void* q, void* scale, uint32_t n, uint32_t batch, void* stream);
+int pdk_quantize_e4m3_blk_bf16(const void* x, void* q, void* scale, uint32_t n, uint32_t batch, void* stream);
+/* x f32 [batch][n] += proj (NULL: no residual), written back when there is one; xn f32 = x * (1 / sqrtf(mean(x^2) + eps)) * w (NULL: not
+ * wanted); q, scale = the quantizer on that.  n % 4 == 0, f32 rows on 16-byte boundaries; 801 for n > 65536. */
+int pdk_add_rmsnorm_quant_e4m3_blk(void* x, const void* proj, const void* w, void* xn, void* q, void* scale, uint32_t n, float eps,
+                                   uint32_t batch, void* stream);
+/* load time: weights bf16 [out][in] -> data, scale (any sizes), and y f32 [out][in] = code * scale */
+int pdk_bf16_to_f8blk(const void* bf16, void* data, void* scale, uint32_t in_dim, uint32_t out_dim, void* stream);
+int pdk_f8blk_dequant(const void* data, const void* scale, void* y, uint32_t in_dim, uint32_t out_dim, void* stream);
+/* y f32 / bf16 [batch][out] = sum over blocks b of x_scale[t][b] * w_scale[o/128][b] * (the block's product of codes), f32 sums.  Any
+ * batch and out_dim; in_dim % 16 == 0, data and xq on 16-byte boundaries. */
+int pdk_f8blk_gemm(const void* data, const void* w_scale, const void* xq, const void* x_scale, void* y, uint32_t in_dim,
+                   uint32_t out_dim, uint32_t batch, void* stream);
+int pdk_f8blk_gemm_bf16(const void* data, const void* w_scale, const void* xq, const void* x_scale, void* y, uint32_t in_dim,
+                        uint32_t out_dim, uint32_t batch, void* stream);
+/* The front of a gated feed-forward block in one kernel: g, u = the products of two planes [ff][in]; h = g / (1 + exp(-g)) * u in f32,
+ * left quantized as the down projection reads it: hq e4m3 [batch][ff], h_scale f32 [batch][ceil(ff/128)].  in_dim % 16 == 0,
+ * ff % 16 == 0; data, xq and hq on 16-byte boundaries. */
+int pdk_f8blk_gate_up(const void* gate_data, const void* gate_scale, const void* up_data, const void* up_scale, const void* xq,
+                      const void* x_scale, void* hq, void* h_scale, uint32_t in_dim, uint32_t ff, uint32_t batch, void* stream);
+
 /* ---- NVFP4: e2m1 nibbles (low nibble = even k), e4m3 scale per 16, f32 scale2 per tensor --- */
 
 /* slot 119, packs/cuda/src/quant/nvf4.cuh:405-421 (rules quant/e2m1.cuh:12-41): f32 x[n] ->

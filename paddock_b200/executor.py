@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 
 ERRORS = ["Ok", "MissingOp", "NoKernel", "Unsupported", "Driver", "Launch", "Pack", "Format"]
-PLANE_KINDS = ["Raw", "Q8", "Kq", "F8Row", "Nvf4", "Mxfp4"]
+PLANE_KINDS = ["Raw", "Q8", "Kq", "F8Row", "Nvf4", "Mxfp4", "F8Blk"]
 NVF4_LAYOUTS = ["Row", "Tiled", "Frag"]
 
 
@@ -181,6 +181,19 @@ class GpuExecutor:
         return self._plane(_lib().pdx_f8row_upload, p, s.ctypes.data_as(C.POINTER(C.c_float)), C.c_uint64(in_dim),
                            C.c_uint64(out_dim))
 
+    def bf16_to_f8blk(self, bf16_bits, in_dim, out_dim):
+        """bf16 weights -> e4m3 with a scale per 128 x 128 tile."""
+        p, n, keep = _host(bf16_bits)
+        assert n == in_dim * out_dim * 2
+        return self._plane(_lib().pdx_bf16_to_f8blk, p, C.c_uint64(in_dim), C.c_uint64(out_dim))
+
+    def f8blk_upload(self, e4m3, scales, in_dim, out_dim):
+        p, n, keep = _host(e4m3)
+        s = np.ascontiguousarray(scales, np.float32)
+        assert n == in_dim * out_dim and s.size == -(-out_dim // 128) * -(-in_dim // 128)
+        return self._plane(_lib().pdx_f8blk_upload, p, s.ctypes.data_as(C.POINTER(C.c_float)), C.c_uint64(in_dim),
+                           C.c_uint64(out_dim))
+
     def nvf4_upload(self, packed, scales, scale2, out_dim, in_dim):
         p, n, keep = _host(packed)
         s, sn, keep2 = _host(scales)
@@ -223,6 +236,22 @@ class GpuExecutor:
 
     def f8row_gemm(self, w, xq, xrs, y, batch):
         self._check(_lib().pdx_f8row_gemm(self._h, w._h, _ptr(xq), _ptr(xrs), _ptr(y), C.c_uint32(batch)))
+
+    def quantize_e4m3_blk(self, x, q, scale, n, batch):
+        self._check(_lib().pdx_quantize_e4m3_blk(self._h, _ptr(x), _ptr(q), _ptr(scale), C.c_uint32(n), C.c_uint32(batch)))
+
+    def add_rmsnorm_quant_e4m3_blk(self, x, proj, w, xn, q, scale, n, eps, batch):
+        self._check(_lib().pdx_add_rmsnorm_quant_e4m3_blk(self._h, _ptr(x), _ptr(proj), _ptr(w), _ptr(xn), _ptr(q), _ptr(scale),
+                                                          C.c_uint32(n), C.c_float(eps), C.c_uint32(batch)))
+
+    def f8blk_dequant(self, w, out):
+        self._check(_lib().pdx_f8blk_dequant(self._h, w._h, _ptr(out)))
+
+    def f8blk_gemm(self, w, xq, xs, y, batch):
+        self._check(_lib().pdx_f8blk_gemm(self._h, w._h, _ptr(xq), _ptr(xs), _ptr(y), C.c_uint32(batch)))
+
+    def f8blk_gate_up(self, gate, up, xq, xs, hq, hs, batch):
+        self._check(_lib().pdx_f8blk_gate_up(self._h, gate._h, up._h, _ptr(xq), _ptr(xs), _ptr(hq), _ptr(hs), C.c_uint32(batch)))
 
     def quantize_nvf4(self, x, q, scale, n):
         self._check(_lib().pdx_quantize_nvf4(self._h, _ptr(x), _ptr(q), _ptr(scale), C.c_uint32(n)))

@@ -56,6 +56,12 @@ struct PdxExecutor {
     void* slot[PDK_TABLE_SLOTS] = {};
     // named exports outside the table
     decltype(&pdk_kquant_gemm_f32) kquant_gemm_f32 = nullptr;
+    decltype(&pdk_quantize_e4m3_blk) quantize_e4m3_blk = nullptr;
+    decltype(&pdk_add_rmsnorm_quant_e4m3_blk) add_rmsnorm_quant_e4m3_blk = nullptr;
+    decltype(&pdk_bf16_to_f8blk) bf16_to_f8blk = nullptr;
+    decltype(&pdk_f8blk_dequant) f8blk_dequant = nullptr;
+    decltype(&pdk_f8blk_gemm) f8blk_gemm = nullptr;
+    decltype(&pdk_f8blk_gate_up) f8blk_gate_up = nullptr;
     DevBuf staging;
     size_t staging_cap = 128u << 20;
     std::mutex mu;
@@ -297,6 +303,12 @@ PDX_EXPORT int pdx_open(const char* pack_path, int device, PdxExecutor** out, ch
     const size_t n = ((size_t)table->size < (size_t)PDK_TABLE_BYTES ? (size_t)table->size : (size_t)PDK_TABLE_BYTES) - 8u;
     memcpy(ex->slot, table->slot, n);
     ex->kquant_gemm_f32 = (decltype(&pdk_kquant_gemm_f32))dlsym(lib, "pdk_kquant_gemm_f32");
+    ex->quantize_e4m3_blk = (decltype(&pdk_quantize_e4m3_blk))dlsym(lib, "pdk_quantize_e4m3_blk");
+    ex->add_rmsnorm_quant_e4m3_blk = (decltype(&pdk_add_rmsnorm_quant_e4m3_blk))dlsym(lib, "pdk_add_rmsnorm_quant_e4m3_blk");
+    ex->bf16_to_f8blk = (decltype(&pdk_bf16_to_f8blk))dlsym(lib, "pdk_bf16_to_f8blk");
+    ex->f8blk_dequant = (decltype(&pdk_f8blk_dequant))dlsym(lib, "pdk_f8blk_dequant");
+    ex->f8blk_gemm = (decltype(&pdk_f8blk_gemm))dlsym(lib, "pdk_f8blk_gemm");
+    ex->f8blk_gate_up = (decltype(&pdk_f8blk_gate_up))dlsym(lib, "pdk_f8blk_gate_up");
     if (const char* cap = getenv("PADDOCK_STAGING_MAX")) {
         const long long v = atoll(cap);
         if (v > 0) ex->staging_cap = (size_t)v;
@@ -602,6 +614,51 @@ PDX_EXPORT int pdx_f8row_upload(PdxExecutor* ex, const void* e4m3, const float* 
     return PDX_OK;
 }
 
+namespace {
+// An F8Blk plane whose data (in_dim * out_dim bytes) and scales `fill` writes.
+template <typename Fill>
+int make_f8blk(PdxExecutor* ex, uint64_t in_dim, uint64_t out_dim, PdxPlane** out, Fill fill) {
+    if (in_dim == 0 || out_dim == 0 || in_dim % 16u != 0 || in_dim > 0x7fffff00ull || out_dim > 0x7fffff00ull)
+        return ex->fail(PDX_UNSUPPORTED, "f8blk plane [%llu, %llu]: in_dim must be a multiple of 16", (unsigned long long)out_dim,
+                        (unsigned long long)in_dim);
+    PdxPlane* p = new PdxPlane();
+    p->kind = PDX_PLANE_F8BLK;
+    p->in_dim = in_dim;
+    p->out_dim = out_dim;
+    int rc = fill(p, (in_dim + 127u) / 128u * ((out_dim + 127u) / 128u) * 4u);
+    if (rc != PDX_OK) {
+        pdx_plane_free(ex, p);
+        return rc;
+    }
+    *out = p;
+    return PDX_OK;
+}
+}  // namespace
+
+PDX_EXPORT int pdx_bf16_to_f8blk(PdxExecutor* ex, const void* bf16, uint64_t in_dim, uint64_t out_dim, PdxPlane** out) {
+    if (!out || !bf16) return PDX_UNSUPPORTED;
+    *out = nullptr;
+    if (!ex->bf16_to_f8blk) return ex->fail(PDX_MISSING_OP, "pdk_bf16_to_f8blk");
+    return make_f8blk(ex, in_dim, out_dim, out, [&](PdxPlane* p, uint64_t scale_bytes) {
+        int rc = ex->alloc(in_dim * out_dim, &p->data, "f8blk data plane");
+        if (rc == PDX_OK) rc = ex->alloc(scale_bytes, &p->scale, "f8blk scale plane");
+        if (rc != PDX_OK) return rc;
+        return ex->with_staged_raw(bf16, in_dim * out_dim * 2u, [&](void* sp) {
+            return ex->launched(ex->bf16_to_f8blk(sp, p->data.p, p->scale.p, (uint32_t)in_dim, (uint32_t)out_dim, ex->stream), "pdk_bf16_to_f8blk");
+        });
+    });
+}
+
+PDX_EXPORT int pdx_f8blk_upload(PdxExecutor* ex, const void* e4m3, const float* scales, uint64_t in_dim, uint64_t out_dim, PdxPlane** out) {
+    if (!out || !e4m3 || !scales) return PDX_UNSUPPORTED;
+    *out = nullptr;
+    return make_f8blk(ex, in_dim, out_dim, out, [&](PdxPlane* p, uint64_t scale_bytes) {
+        int rc = ex->clone_htod(e4m3, in_dim * out_dim, &p->data, "f8blk data plane");
+        if (rc == PDX_OK) rc = ex->clone_htod(scales, scale_bytes, &p->scale, "f8blk scale plane");
+        return rc;
+    });
+}
+
 PDX_EXPORT int pdx_nvf4_upload(PdxExecutor* ex, const void* packed, uint64_t packed_len, const void* scales,
                                uint64_t scales_len, float scale2, uint64_t out_dim, uint64_t in_dim, PdxPlane** out) {
     if (!out || !packed || !scales) return PDX_UNSUPPORTED;
@@ -765,6 +822,42 @@ PDX_EXPORT int pdx_f8row_gemm(PdxExecutor* ex, const PdxPlane* w, const void* xq
     if (!f) return ex->fail(PDX_MISSING_OP, "f8row_gemm");
     return ex->launched(f(w->data.p, w->scale.p, xq, xrs, y, (uint32_t)w->in_dim, (uint32_t)w->out_dim, batch, ex->stream),
                         "f8row_gemm");
+}
+
+PDX_EXPORT int pdx_quantize_e4m3_blk(PdxExecutor* ex, const void* x, void* q, void* scale, uint32_t n, uint32_t batch) {
+    if (!ex->quantize_e4m3_blk) return ex->fail(PDX_MISSING_OP, "pdk_quantize_e4m3_blk");
+    return ex->launched(ex->quantize_e4m3_blk(x, q, scale, n, batch, ex->stream), "pdk_quantize_e4m3_blk");
+}
+
+PDX_EXPORT int pdx_add_rmsnorm_quant_e4m3_blk(PdxExecutor* ex, void* x, const void* proj, const void* w, void* xn, void* q, void* scale,
+                                              uint32_t n, float eps, uint32_t batch) {
+    if (!ex->add_rmsnorm_quant_e4m3_blk) return ex->fail(PDX_MISSING_OP, "pdk_add_rmsnorm_quant_e4m3_blk");
+    return ex->launched(ex->add_rmsnorm_quant_e4m3_blk(x, proj, w, xn, q, scale, n, eps, batch, ex->stream), "pdk_add_rmsnorm_quant_e4m3_blk");
+}
+
+PDX_EXPORT int pdx_f8blk_dequant(PdxExecutor* ex, const PdxPlane* w, void* out_f32) {
+    if (!w || w->kind != PDX_PLANE_F8BLK) return ex->fail(PDX_UNSUPPORTED, "f8blk_dequant needs an F8Blk plane");
+    if (!ex->f8blk_dequant) return ex->fail(PDX_MISSING_OP, "pdk_f8blk_dequant");
+    return ex->launched(ex->f8blk_dequant(w->data.p, w->scale.p, out_f32, (uint32_t)w->in_dim, (uint32_t)w->out_dim, ex->stream),
+                        "pdk_f8blk_dequant");
+}
+
+PDX_EXPORT int pdx_f8blk_gemm(PdxExecutor* ex, const PdxPlane* w, const void* xq, const void* xs, void* y, uint32_t batch) {
+    if (!w || w->kind != PDX_PLANE_F8BLK) return ex->fail(PDX_UNSUPPORTED, "f8blk_gemm needs an F8Blk plane");
+    if (!ex->f8blk_gemm) return ex->fail(PDX_MISSING_OP, "pdk_f8blk_gemm");
+    return ex->launched(ex->f8blk_gemm(w->data.p, w->scale.p, xq, xs, y, (uint32_t)w->in_dim, (uint32_t)w->out_dim, batch, ex->stream),
+                        "pdk_f8blk_gemm");
+}
+
+PDX_EXPORT int pdx_f8blk_gate_up(PdxExecutor* ex, const PdxPlane* gate, const PdxPlane* up, const void* xq, const void* xs, void* hq, void* hs,
+                                 uint32_t batch) {
+    if (!gate || gate->kind != PDX_PLANE_F8BLK || !up || up->kind != PDX_PLANE_F8BLK)
+        return ex->fail(PDX_UNSUPPORTED, "f8blk_gate_up needs two F8Blk planes");
+    if (gate->in_dim != up->in_dim || gate->out_dim != up->out_dim) return ex->fail(PDX_UNSUPPORTED, "f8blk_gate_up: planes of different sizes");
+    if (!ex->f8blk_gate_up) return ex->fail(PDX_MISSING_OP, "pdk_f8blk_gate_up");
+    return ex->launched(ex->f8blk_gate_up(gate->data.p, gate->scale.p, up->data.p, up->scale.p, xq, xs, hq, hs, (uint32_t)gate->in_dim,
+                                          (uint32_t)gate->out_dim, batch, ex->stream),
+                        "pdk_f8blk_gate_up");
 }
 
 PDX_EXPORT int pdx_quantize_nvf4(PdxExecutor* ex, const void* x, void* q, void* scale, uint32_t n) {

@@ -121,6 +121,14 @@ _EXTRA_SIGS = {
     "pdk_kquant_gemm_f32": "ppppuuuu",
     "pdk_f8row_gemm_bf16": "pppppuuu",
     "pdk_nvf4_gemm_bf16": "ppppppfuuu",
+    "pdk_quantize_e4m3_blk": "pppuu",
+    "pdk_quantize_e4m3_blk_bf16": "pppuu",
+    "pdk_add_rmsnorm_quant_e4m3_blk": "ppppppufu",
+    "pdk_bf16_to_f8blk": "pppuu",
+    "pdk_f8blk_dequant": "pppuu",
+    "pdk_f8blk_gemm": "pppppuuu",
+    "pdk_f8blk_gemm_bf16": "pppppuuu",
+    "pdk_f8blk_gate_up": "ppppppppuuu",
     "pdk_moe_prep_act": "pppuu",
     "pdk_mxfp4_moe_gate_up": "pppppppppppuuuuff",
     "pdk_mxfp4_moe_down": "ppppppppppuuuuu",

@@ -84,6 +84,82 @@ class GpuExecutor:
                        stream=_stream())
 
 
+    # -- block-scaled e4m3 (no counterpart in the reference) -------------------------------
+    def bf16_to_f8blk(self, w, in_dim, out_dim):
+        """bf16 weights [out][in] on the device -> F8BlkPlane."""
+        data = torch.empty(out_dim * in_dim, dtype=torch.uint8, device=self.device)
+        scale = torch.empty(_blocks(out_dim) * _blocks(in_dim), dtype=torch.float32, device=self.device)
+        self.pack.call("pdk_bf16_to_f8blk", w, data, scale, in_dim, out_dim, stream=_stream())
+        return F8BlkPlane(data, scale, (in_dim, out_dim))
+
+    def f8blk_dequant(self, w, y):
+        self.pack.call("pdk_f8blk_dequant", w.data, w.scale, y, w.dims[0], w.dims[1], stream=_stream())
+
+    def quantize_e4m3_blk(self, x, q, scale, n, batch):
+        """x f32 or bf16 [batch][n] -> codes and a scale per token and 128 elements."""
+        self.pack.call(_by_type(x, "pdk_quantize_e4m3_blk"), x, q, scale, n, batch, stream=_stream())
+
+    def add_rmsnorm_quant_e4m3_blk(self, x, proj, w, xn, q, scale, n, eps, batch):
+        """x += proj (None: no residual); xn = rmsnorm(x) * w (None: not wanted); codes and scales of that."""
+        self.pack.call("pdk_add_rmsnorm_quant_e4m3_blk", x, proj, w, xn, q, scale, n, eps, batch, stream=_stream())
+
+    def f8blk_gemm(self, w, xq, xs, y, batch):
+        """y f32 or bf16 [batch][out]."""
+        self.pack.call(_by_type(y, "pdk_f8blk_gemm"), w.data, w.scale, xq, xs, y, w.dims[0], w.dims[1], batch, stream=_stream())
+
+    def f8blk_gate_up(self, gate, up, xq, xs, hq, hs, batch):
+        """Codes and scales of silu(x . Wg^T) * (x . Wu^T)."""
+        if gate.dims != up.dims:
+            raise ValueError(f"gate plane {gate.dims} and up plane {up.dims} differ")
+        self.pack.call("pdk_f8blk_gate_up", gate.data, gate.scale, up.data, up.scale, xq, xs, hq, hs, gate.dims[0], gate.dims[1], batch,
+                       stream=_stream())
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _by_type(t, name):
+    """The f32 or the bf16 form of a call."""
+    if t.dtype == torch.float32:
+        return name
+    if t.dtype == torch.bfloat16:
+        return name + "_bf16"
+    raise TypeError(f"{name} takes f32 or bf16, not {t.dtype}")
+
+
+@dataclass
+class F8BlkPlane:
+    """e4m3 data [out][in] + one f32 scale per 128 x 128 tile [ceil(out/128)][ceil(in/128)]; dims = (in, out)."""
+    data: torch.Tensor
+    scale: torch.Tensor
+    dims: tuple
+
+
+class F8BlkFfnWorkspace:
+    """Buffers of one gated feed-forward block over F8BlkPlanes, for up to `tokens` tokens (allocated once, reused)."""
+
+    def __init__(self, ex, embd, ff, tokens):
+        self.tokens = tokens
+        self.xq = torch.empty(tokens * embd, dtype=torch.uint8, device=ex.device)
+        self.xs = torch.empty(tokens * _blocks(embd), dtype=torch.float32, device=ex.device)
+        self.hq = torch.empty(tokens * ff, dtype=torch.uint8, device=ex.device)
+        self.hs = torch.empty(tokens * _blocks(ff), dtype=torch.float32, device=ex.device)
+
+
+def ffn_f8blk_forward(ex, gate, up, down, ws, x, proj, norm, eps, y, batch):
+    """x += proj, then y = down(silu(gate(h)) * up(h)) of h = rmsnorm(x) * norm: residual add, norm and quantizer, the gated front,
+    the down projection, one launch each.  y (f32 or bf16 [batch][embd]) is the next call's proj when it is f32."""
+    embd = gate.dims[0]
+    if down.dims != (gate.dims[1], embd):
+        raise ValueError(f"down plane {down.dims} does not follow gate plane {gate.dims}")
+    if batch > ws.tokens:
+        raise ValueError(f"{batch} tokens in a workspace of {ws.tokens}")
+    ex.add_rmsnorm_quant_e4m3_blk(x, proj, norm, None, ws.xq, ws.xs, embd, eps, batch)
+    ex.f8blk_gate_up(gate, up, ws.xq, ws.xs, ws.hq, ws.hs, batch)
+    ex.f8blk_gemm(down, ws.hq, ws.hs, y, batch)
+
+
 @dataclass
 class RepackedMxfp4:
     """types.rs:111-127: 16-byte nibble blocks + 1-byte E8M0 scales."""
