@@ -1,0 +1,51 @@
+// f8blk_tc5.cuh - what the two tensor-core kernels of block-scaled e4m3 products share.
+//
+// The scales of a block are arbitrary f32, so the tensor core cannot apply them: it sums one 128-element block of K at a time into
+// tensor memory (kind::f8f6f4, f32), and the epilogue warps, which keep the product in registers, add it on with the block's
+// two scales while the tensor core does the next block.  That costs one fused multiply-add per element and block, and reading every
+// element of tensor memory once per block.
+#pragma once
+#include "f8blk.cuh"
+#include "tc5.cuh"
+
+namespace f8blk {
+
+// One plane or, for the gated front, two; y = f32 / bf16 product, or hq with hs.
+struct Call {
+    const void *w[2], *ws[2], *xq, *xs;
+    void *y, *hs;
+    uint32_t in_dim, out_dim, batch;
+};
+
+// tensor memory -> registers: 32 lanes x 16 columns of 32 bits per warp
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// two f32 in one register pair, and acc += v * s on both: half the issue slots of two fused multiply-adds, same roundings
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    uint32_t lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
+}
+
+__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+}  // namespace f8blk
+
+// f8blk_split.cu, f8blk_pair.cu: 0 or a cudaError_t
+int pdk_f8blk_split(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
+int pdk_f8blk_pair(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
