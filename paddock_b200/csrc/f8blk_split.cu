@@ -143,7 +143,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
         uint32_t stage = 0, phase = 0;
         for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
             if (kb - kb_lo >= pre) {
-                ok = __all_sync(0xffffffffu, tc5::mbar_wait(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, stage));
+                ok = __all_sync(0xffffffffu, wait_soon(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, stage));
                 if (!ok) break;
                 issue_w(stage, kb);
             }
@@ -157,8 +157,8 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
         // ------------------------------------------------------------ MMA issuer (whole warp, one lane issues)
         uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
         for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
-            ok = __all_sync(0xffffffffu, tc5::mbar_wait(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf) &&
-                                             tc5::mbar_wait(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage));
+            ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf) &&
+                                             wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage));
             if (!ok) break;
             tc5::fence_after_sync();
             const uint32_t s_addr = tc5::smem_u32(smem + stage * C::kStageBytes);
@@ -203,7 +203,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             }
             if (kb + 1u < kb_hi) fetch(kb + 1u);
             __syncwarp();
-            ok = __all_sync(0xffffffffu, tc5::mbar_wait(&sh->acc_full[buf], bphase, ctx, tc5::kErrTmemFullWait, buf));
+            ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_full[buf], bphase, ctx, tc5::kErrTmemFullWait, buf));
             if (!ok) break;
             tc5::fence_after_sync();
 #pragma unroll

@@ -17,6 +17,13 @@ struct Call {
     uint32_t in_dim, out_dim, batch;
 };
 
+// tc5::mbar_wait that reads the global timer only after some failed attempts: these waits are short and one per block of K.
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const tc5::WaitCtx& ctx, unsigned int code, unsigned int detail) {
+    for (uint32_t i = 0; i < 64u; ++i)
+        if (tc5::mbar_try_wait(bar, parity)) return true;
+    return tc5::mbar_wait(bar, parity, ctx, code, detail);
+}
+
 // tensor memory -> registers: 32 lanes x 16 columns of 32 bits per warp
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -27,7 +34,25 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         : "memory");
 }
 
-// two f32 in one register pair, and acc += v * s on both: half the issue slots of two fused multiply-adds, same roundings
+// The wait for this warp's loads, as what hands their registers on: nothing that uses them can be moved in front of it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+// two f32 in one register pair, and acc += v * s on both: the roundings of two fused multiply-adds
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     uint64_t d;
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
@@ -42,10 +67,12 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
 }
 
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u.  The quotient is the hardware's (2 units, 0 where exp(-g) passes 2^126): an IEEE one has a rare path that is branched
+// to, which keeps neighbouring elements from overlapping.
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 }  // namespace f8blk
 
-// f8blk_split.cu, f8blk_pair.cu: 0 or a cudaError_t
+// f8blk_split.cu, f8blk_wide.cu: 0 or a cudaError_t
 int pdk_f8blk_split(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
-int pdk_f8blk_pair(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
+int pdk_f8blk_wide(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);

@@ -1,0 +1,341 @@
+// f8blk_wide.cu - products of block-scaled e4m3 operands at prompt widths.
+//
+// Persistent CTAs, one per SM, tiles of 128 tokens x 256 channels (tcgen05, M = 128 x N = 256 x K = 32 per instruction).  Tokens are
+// the lanes, so a thread owns one token, and a block's two scales are one number per thread: the block's sums come out of tensor
+// memory and go onto the product with one fused multiply-add each.
+//
+//   warp 0      producer: a block of K of the tokens (16 KB) and of the channels (32 KB) per stage
+//   warp 1      MMA issuer: four MMAs per block into one of two buffers of 256 tensor-memory columns
+//   warps 2, 3  the scales: of 64 tokens each, times those of the two halves of the channels, into shared memory.  They arrive on the stage's
+//               barrier like the boxes, so whoever has a block's sums has its scales, without a wait of its own
+//   warps 4..11 the product: warp w has tokens 32 (w % 4) .. + 31 and 128 of the 256 columns, 128 registers a thread, and 64 more for columns on
+//               their way; the first four warps hand registers over for that
+//
+// Gated front: the first 128 channels of a tile are gate's, the others up's beside them.  A warp's columns are then 64 of gate's and the
+// same 64 of up's, so a thread gates its own sums; only the maximum of a token's block crosses to the other half's warp.
+//
+// What bounds it (cycles per block of a tile; 4096 tokens, 5120 x 17408): the tensor core needs 514, loads and additions from
+// tensor memory by themselves 357, the two with their hand-over 630 with operands in place, boxes from L2 (48 KB) 730 without the additions;
+// all together 830, 343 us, 2.1 PFLOP/s.  On the way there:
+//   scales read from global memory by the eight warps, 32 sectors a load              +330 cycles
+//   brought by warps 2 and 3, but under barriers of their own                         +170
+//   packed multiply-adds (fma.rn.f32x2): the pairs are moved together first           +200
+//   pairs of SMs (cta_group::2, two thirds of the L2 traffic): every block crosses between the SMs twice, and the barriers of two CTAs in
+//   lock step cost what the traffic saves: 377 us at best
+// Every wait is bounded; a role that gives up goes on through the loop without waiting or touching memory, so that the named
+// barriers of the others meet.
+#include "f8blk_tc5.cuh"
+
+namespace {
+
+using namespace f8blk;
+
+constexpr uint32_t BM = 128, BN = 256, BNH = 128, BK = 128;   // tokens, channels, channels of a half, K per stage
+constexpr uint32_t kStages = 4;
+constexpr uint32_t kABytes = BM * BK, kBHalf = BNH * BK, kStageBytes = kABytes + 2u * kBHalf;
+constexpr uint32_t kWarps = 8, kFirst = 4;                    // that keep the product, and the first of them
+constexpr uint32_t kThreads = (kFirst + kWarps) * 32u;
+// registers a thread: 168 at launch (64,512 in all), 56 for the first four warps and 224 for the others after the split (64,512)
+constexpr uint32_t kRegsFew = 56, kRegsMany = 224;
+static_assert(kFirst * 32u * kRegsFew + kWarps * 32u * kRegsMany <= kThreads * 168u, "the split draws on what the launch has");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kAhead = 4;                                // blocks whose scales a lane loads together
+// Scales are written when a stage is free and read when its sums are: at most the stages and the two buffers lie between.
+constexpr uint32_t kSlots = 8;
+static_assert(kStages + 2u <= kSlots, "a slot is written again after it was read");
+
+struct Shared {
+    uint64_t full[kStages];
+    uint64_t empty[kStages];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    float amax[2][BM];
+    float scale[kSlots][2][BM];      // block % kSlots: the products of the scales, per half of the channels and token
+};
+
+struct Args {
+    const float *ws0, *ws1, *xs;
+    void* y;
+    float* hs;
+    uint32_t out_dim, batch, num_kb;
+    uint32_t row_align;              // bytes, 32, 16 or less, that every row of y starts on
+    unsigned int* err;
+};
+
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y),
+                 "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+// 16 bytes of a row: 4 f32 or 8 bf16
+__device__ __forceinline__ uint4 piece(const float* v, float*) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ uint4 piece(const float* v, __nv_bfloat16*) {
+    return make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+}
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// a thread's 128 channels of its token's row, `left` of which the row has
+template <typename TO>
+__device__ __forceinline__ void store_row(TO* out, const float (&v)[BNH], uint32_t left, uint32_t align) {
+    constexpr uint32_t kPer = 16u / sizeof(TO);
+    if (align >= 16u) {       // rows end on a piece too
+        const bool wide = align >= 32u;
+#pragma unroll
+        for (uint32_t i = 0; i < BNH; i += 2u * kPer) {
+            const uint4 a = piece(v + i, out), b = piece(v + i + kPer, out);
+            if (wide) {
+                if (i < left) store32(out + i, a, b);
+            } else {
+                if (i < left) *reinterpret_cast<uint4*>(out + i) = a;
+                if (i + kPer < left) *reinterpret_cast<uint4*>(out + i + kPer) = b;
+            }
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < BNH; ++i)
+            if (i < left) put(out + i, v[i]);
+    }
+}
+
+template <int kPlanes, typename TO>
+__global__ void __launch_bounds__(kThreads, 1)
+f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w0,
+                  const __grid_constant__ CUtensorMap tmap_w1, const Args a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
+    Shared* sh = reinterpret_cast<Shared*>(tiles + kStages * kStageBytes);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    constexpr uint32_t kTileN = kPlanes == 2 ? BNH : BN;      // channels of y (of h) per tile
+    const uint32_t tiles_m = (a.batch + BM - 1u) / BM, tiles_n = (a.out_dim + kTileN - 1u) / kTileN;
+    const uint32_t n_tiles = tiles_m * tiles_n, w_blocks = (a.out_dim + 127u) / 128u;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            tc5::mbar_init(&sh->full[s], 3);     // the expected-bytes arrival, two warps of scales
+            tc5::mbar_init(&sh->empty[s], 1);
+        }
+        for (uint32_t b = 0; b < 2; ++b) {
+            tc5::mbar_init(&sh->acc_full[b], 1);
+            tc5::mbar_init(&sh->acc_empty[b], kWarps);
+        }
+        sh->abort_flag = 0;
+        tc5::mbar_fence_init();
+        tc5::tma_prefetch_desc(&tmap_x);
+        tc5::tma_prefetch_desc(&tmap_w0);
+        if (kPlanes == 2) tc5::tma_prefetch_desc(&tmap_w1);
+    }
+    if (warp == 1u) {
+        tc5::tmem_alloc(&sh->tmem_base, kTmemCols);
+        tc5::tmem_relinquish();
+    }
+    tc5::fence_before_sync();
+    __syncthreads();
+    tc5::fence_after_sync();
+    const uint32_t tmem_base = sh->tmem_base;
+    const tc5::WaitCtx ctx{&sh->abort_flag, a.err};
+    pdk_pdl_launch_dependents();
+
+    if (warp < kFirst) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+        bool ok = true;
+        if (warp == 0u) {
+            // -------------------------------------------------------- TMA producer (whole warp, one lane issues)
+            uint32_t stage = 0, phase = 0;
+            pdk_pdl_wait();
+            for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
+                const uint32_t m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * kTileN;
+                for (uint32_t kb = 0; kb < a.num_kb; ++kb) {
+                    ok = __all_sync(0xffffffffu, wait_soon(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, stage));
+                    if (!ok) break;
+                    uint8_t* s = tiles + stage * kStageBytes;
+                    tc5::mbar_arrive_expect_tx_elect(&sh->full[stage], kStageBytes);
+                    tc5::tma_load_2d_elect(s, &tmap_x, &sh->full[stage], (int32_t)(kb * BK), (int32_t)m0);
+                    tc5::tma_load_2d_elect(s + kABytes, &tmap_w0, &sh->full[stage], (int32_t)(kb * BK), (int32_t)n0);
+                    tc5::tma_load_2d_elect(s + kABytes + kBHalf, kPlanes == 2 ? &tmap_w1 : &tmap_w0, &sh->full[stage], (int32_t)(kb * BK),
+                                           (int32_t)(kPlanes == 2 ? n0 : n0 + BNH));
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok && lane == 0)
+                for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies in flight still land in this CTA
+            __syncwarp();
+        } else if (warp == 1u) {
+            // -------------------------------------------------------- MMA issuer (whole warp, one lane issues)
+            constexpr uint32_t idesc = tc5::idesc_f32acc(0u, 0u, BM, BN);
+            uint32_t stage = 0, phase = 0, block = 0;
+            for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x)
+                for (uint32_t kb = 0; kb < a.num_kb; ++kb, ++block) {
+                    const uint32_t buf = block & 1u, bphase = (block >> 1) & 1u;
+                    ok = __all_sync(0xffffffffu, wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage) &&
+                                                     wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf));
+                    if (!ok) break;
+                    tc5::fence_after_sync();
+                    const uint32_t a_addr = tc5::smem_u32(tiles + stage * kStageBytes);
+                    tc5::mma_f8f6f4_x4_elect(tmem_base + buf * BN, tc5::smem_desc_sw128(a_addr), tc5::smem_desc_sw128(a_addr + kABytes), idesc, 0u);
+                    tc5::mma_commit_elect(&sh->acc_full[buf]);
+                    tc5::mma_commit_elect(&sh->empty[stage]);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            pdk_pdl_wait();
+        } else {
+            // -------------------------------------------------------- scales
+            const uint32_t row = (warp - 2u) * 64u + lane;
+            uint32_t stage = 0, phase = 0, block = 0;
+            pdk_pdl_wait();
+            for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
+                const uint32_t t = (tile % tiles_m) * BM + row, nb = (tile / tiles_m) * kTileN / 128u;
+                const float* x0 = a.xs + (size_t)min(t, a.batch - 1u) * a.num_kb;
+                const float* x1 = a.xs + (size_t)min(t + 32u, a.batch - 1u) * a.num_kb;
+                const float* w0 = a.ws0 + (size_t)nb * a.num_kb;
+                const float* w1 = kPlanes == 2 ? a.ws1 + (size_t)nb * a.num_kb : a.ws0 + (size_t)min(nb + 1u, w_blocks - 1u) * a.num_kb;
+                for (uint32_t k0 = 0; k0 < a.num_kb && ok; k0 += kAhead) {
+                    float x[2][kAhead], w[2][kAhead];
+#pragma unroll
+                    for (uint32_t j = 0; j < kAhead; ++j) {
+                        const uint32_t kb = min(k0 + j, a.num_kb - 1u);
+                        x[0][j] = x0[kb]; x[1][j] = x1[kb]; w[0][j] = w0[kb]; w[1][j] = w1[kb];
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < kAhead; ++j) {
+                        if (k0 + j >= a.num_kb || !ok) break;
+                        ok = __all_sync(0xffffffffu, wait_soon(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, 16u + stage));
+                        if (!ok) break;
+                        float(&slot)[2][BM] = sh->scale[block++ % kSlots];
+#pragma unroll
+                        for (uint32_t h = 0; h < 2u; ++h) {
+                            slot[h][row] = x[0][j] * w[h][j];
+                            slot[h][row + 32u] = x[1][j] * w[h][j];
+                        }
+                        __syncwarp();
+                        if (lane == 0u) tc5::mbar_arrive(&sh->full[stage]);
+                        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
+        // ------------------------------------------------------------ the product
+        const uint32_t quarter = warp & 3u, half = (warp - kFirst) >> 2;
+        const uint32_t row = quarter * 32u + lane;           // token of the tile
+        // columns: 128 in a row, or 64 of gate's and the same of up's
+        const uint32_t lanes = tmem_base + ((quarter * 32u) << 16) + half * (kPlanes == 2 ? 64u : BNH);
+        constexpr uint32_t kSecond = kPlanes == 2 ? BNH : 64u;                // where the second 64 start
+        uint32_t block = 0;
+        bool ok = true;
+        pdk_pdl_wait();
+        for (uint32_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+            const uint32_t m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * kTileN;
+            const uint32_t t = m0 + row;
+            float acc[BNH];
+#pragma unroll
+            for (uint32_t i = 0; i < BNH; ++i) acc[i] = 0.0f;
+            for (uint32_t kb = 0; kb < a.num_kb && ok; ++kb, ++block) {
+                const uint32_t buf = block & 1u, bphase = (block >> 1) & 1u;
+                ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_full[buf], bphase, ctx, tc5::kErrTmemFullWait, buf));
+                if (!ok) break;
+                const float s0 = sh->scale[block % kSlots][kPlanes == 2 ? 0u : half][row], s1 = kPlanes == 2 ? sh->scale[block % kSlots][1][row] : s0;
+                tc5::fence_after_sync();
+                // two loads on their way at a time; the second pair follows the first into its registers
+                uint32_t r[2][32];
+                const uint32_t from = lanes + buf * BN;
+                auto add = [&](uint32_t c) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32u; ++i) acc[c * 32u + i] = fmaf(__uint_as_float(r[c & 1u][i]), c < 2u ? s0 : s1, acc[c * 32u + i]);
+                };
+                tc5::tmem_ld_32x32(from, r[0]);
+                tc5::tmem_ld_32x32(from + 32u, r[1]);
+                tmem_ld_wait(r[0]);
+                tmem_ld_wait(r[1]);
+                add(0u);
+                tc5::tmem_ld_32x32(from + kSecond, r[0]);
+                add(1u);
+                tc5::tmem_ld_32x32(from + kSecond + 32u, r[1]);
+                tmem_ld_wait(r[0]);
+                tmem_ld_wait(r[1]);
+                tc5::fence_before_sync();      // every column is in registers: the buffer goes back
+                __syncwarp();
+                if (lane == 0u) tc5::mbar_arrive(&sh->acc_empty[buf]);
+                add(2u);
+                add(3u);
+            }
+            if constexpr (kPlanes == 1) {
+                const uint32_t n = n0 + half * BNH;
+                if (ok && t < a.batch && n < a.out_dim)
+                    store_row(reinterpret_cast<TO*>(a.y) + (size_t)t * a.out_dim + n, acc, a.out_dim - n, a.row_align);
+            } else {
+                float m = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 64u; ++i) {
+                    acc[i] = gated(acc[i], acc[64u + i]);
+                    m = fmaxf(m, fabsf(acc[i]));
+                }
+                sh->amax[half][row] = m;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float sc = scale_of(fmaxf(m, sh->amax[1u - half][row])), inv = 1.0f / sc;
+                asm volatile("bar.sync 1, 256;" ::: "memory");       // read before the next tile's is written
+                if (ok && t < a.batch) {
+                    const uint32_t n = n0 + half * 64u;
+                    uint8_t* q = reinterpret_cast<uint8_t*>(a.y) + (size_t)t * a.out_dim + n;
+#pragma unroll
+                    for (uint32_t i = 0; i < 64u; i += 16u)
+                        if (n + i < a.out_dim)        // ff % 16 == 0: whole pieces
+                            *reinterpret_cast<uint4*>(q + i) = make_uint4(
+                                codes4(acc[i], acc[i + 1u], acc[i + 2u], acc[i + 3u], inv), codes4(acc[i + 4u], acc[i + 5u], acc[i + 6u], acc[i + 7u], inv),
+                                codes4(acc[i + 8u], acc[i + 9u], acc[i + 10u], acc[i + 11u], inv),
+                                codes4(acc[i + 12u], acc[i + 13u], acc[i + 14u], acc[i + 15u], inv));
+                    if (half == 0u) a.hs[(size_t)t * w_blocks + n0 / 128u] = sc;
+                }
+            }
+        }
+    }
+
+    tc5::fence_before_sync();
+    __syncthreads();
+    if (warp == 1u) {
+        tc5::fence_after_sync();
+        tc5::tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+template <int kPlanes, typename TO>
+int launch_wide(const Call& c, cudaStream_t st) {
+    CUtensorMap tx, tw0, tw1;
+    if (int rc = pdk_make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.xq, c.in_dim, c.batch, c.in_dim, BK, BM)) return rc;
+    if (int rc = pdk_make_tmap_2d(&tw0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[0], c.in_dim, c.out_dim, c.in_dim, BK, BNH)) return rc;
+    tw1 = tw0;
+    if (kPlanes == 2)
+        if (int rc = pdk_make_tmap_2d(&tw1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[1], c.in_dim, c.out_dim, c.in_dim, BK, BNH)) return rc;
+    Args a{};
+    a.ws0 = (const float*)c.ws[0]; a.ws1 = (const float*)c.ws[1]; a.xs = (const float*)c.xs; a.y = c.y; a.hs = (float*)c.hs;
+    a.out_dim = c.out_dim; a.batch = c.batch; a.num_kb = blocks_of(c.in_dim);
+    const uint64_t where = (uint64_t)(uintptr_t)c.y | (uint64_t)c.out_dim * sizeof(TO);
+    a.row_align = where % 32u == 0u ? 32u : where % 16u == 0u ? 16u : (uint32_t)sizeof(TO);
+    a.err = pdk_error_word();
+    const size_t smem = (size_t)kStages * kStageBytes + sizeof(Shared) + 1024u;
+    auto kern = f8blk_wide_kernel<kPlanes, TO>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    const uint32_t tile_n = kPlanes == 2 ? BNH : BN;
+    const uint64_t n_tiles = (uint64_t)((c.batch + BM - 1u) / BM) * ((c.out_dim + tile_n - 1u) / tile_n);
+    if (n_tiles > 0x7fffffffull) return cudaErrorInvalidValue;
+    const uint32_t sms = (uint32_t)pdk_sm_count();
+    return pdk_launch_pdl(kern, dim3(n_tiles < sms ? (uint32_t)n_tiles : sms), dim3(kThreads), smem, st, tx, tw0, tw1, a);
+}
+
+}  // namespace
+
+int pdk_f8blk_wide(const Call& c, int planes, bool bf16, cudaStream_t st) {
+    if (planes == 2) return launch_wide<2, float>(c, st);
+    return bf16 ? launch_wide<1, __nv_bfloat16>(c, st) : launch_wide<1, float>(c, st);
+}
