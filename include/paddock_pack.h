@@ -251,6 +251,9 @@ int pdk_f8blk_gemm_bf16(const void* data, const void* w_scale, const void* xq, c
  * ff % 16 == 0; data, xq and hq on 16-byte boundaries. */
 int pdk_f8blk_gate_up(const void* gate_data, const void* gate_scale, const void* up_data, const void* up_scale, const void* xq,
                       const void* x_scale, void* hq, void* h_scale, uint32_t in_dim, uint32_t ff, uint32_t batch, void* stream);
+/* How pdk_f8blk_gemm (planes 1) or pdk_f8blk_gate_up (planes 2) of this size runs on the current device, for tests and diagnostics:
+ * plan[3] = kernel (1 split over clusters, 2 wide), its tokens (1) or channels (2) a tile, CTAs that share a tile.  0 or a cudaError_t. */
+int pdk_f8blk_plan(uint32_t planes, uint32_t in_dim, uint32_t out_dim, uint32_t batch, uint32_t* plan);
 
 /* ---- NVFP4: e2m1 nibbles (low nibble = even k), e4m3 scale per 16, f32 scale2 per tensor --- */
 

@@ -2,8 +2,8 @@
 //
 //   y[t][n] = sum_b xs[t][b] * ws[n / 128][b] * ( sum_{k in block b} xq[t][k] * wq[n][k] )
 //   h[t][f] = silu(g) * u of two such products, left quantized in blocks of 128 f per token
-#include <cstdlib>
-
+#include "cluster_caps.cuh"
+#include "f8blk_plan.cuh"
 #include "f8blk_tc5.cuh"
 
 namespace {
@@ -14,16 +14,16 @@ bool operands_ok(const void* w, const void* ws, const void* xq, const void* xs, 
            pdk_aligned(w, 16) && pdk_aligned(xq, 16) && pdk_aligned(ws, 4) && pdk_aligned(xs, 4);
 }
 
-// PDK_F8BLK_ROUTE=1 or 2 keeps every call on the split or the wide kernel (A/B switch, read once).
-bool prefer_pair(const f8blk::Call& c, int planes) {
-    static const int force = [] { const char* e = getenv("PDK_F8BLK_ROUTE"); return e ? atoi(e) : 0; }();
-    if (force) return force == 2;
-    if (c.batch <= 128u) return false;
-    const uint64_t small = (uint64_t)((c.batch + 127u) / 128u) * f8blk::blocks_of(c.out_dim) * planes, slabs = f8blk::blocks_of(c.in_dim);
-    return small > 100u && (small - 100u) * slabs > 6000u;
+int plan_of(int planes, uint32_t in_dim, uint32_t out_dim, uint32_t batch, f8blk::Plan* plan) {
+    const uint32_t* resident[2] = {nullptr, nullptr};
+    if (int rc = pdk_f8blk_split_clusters(planes, resident)) return rc;
+    *plan = f8blk::choose(planes, in_dim, out_dim, batch, resident, kPdkMaxCluster, (uint32_t)pdk_sm_count());
+    return 0;
 }
 int launch(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st) {
-    return prefer_pair(c, planes) ? pdk_f8blk_wide(c, planes, bf16, st) : pdk_f8blk_split(c, planes, bf16, st);
+    f8blk::Plan p;
+    if (int rc = plan_of(planes, c.in_dim, c.out_dim, c.batch, &p)) return rc;
+    return p.kernel == 2u ? pdk_f8blk_wide(c, planes, bf16, p.cols, st) : pdk_f8blk_split(c, planes, bf16, p.cols, p.split, st);
 }
 
 int gemm(const void* w, const void* ws, const void* xq, const void* xs, void* y, uint32_t in_dim, uint32_t out_dim, uint32_t batch, bool bf16,
@@ -52,4 +52,13 @@ PDK_EXPORT int pdk_f8blk_gate_up(const void* gate_data, const void* gate_scale, 
         return cudaErrorInvalidValue;
     const f8blk::Call c{{gate_data, up_data}, {gate_scale, up_scale}, xq, x_scale, hq, h_scale, in_dim, ff, batch};
     return launch(c, 2, false, (cudaStream_t)stream);
+}
+
+// Diagnostics: the plan of a product (planes 1) or gated front (planes 2) on the current device
+PDK_EXPORT int pdk_f8blk_plan(uint32_t planes, uint32_t in_dim, uint32_t out_dim, uint32_t batch, uint32_t* plan) {
+    if (planes < 1u || planes > 2u || in_dim == 0u || out_dim == 0u || batch == 0u || !plan) return cudaErrorInvalidValue;
+    f8blk::Plan p;
+    if (int rc = plan_of((int)planes, in_dim, out_dim, batch, &p)) return rc;
+    plan[0] = p.kernel; plan[1] = p.cols; plan[2] = p.split;
+    return 0;
 }

@@ -19,7 +19,6 @@ namespace {
 using namespace f8blk;
 using tc5::cluster_addr;
 using tc5::cluster_sync;
-using tc5::st_cluster;
 
 constexpr uint32_t BM = 128, BK = 128;
 constexpr uint32_t kABytes = BM * BK;
@@ -75,6 +74,9 @@ __device__ __forceinline__ void store_if(__nv_bfloat16* p, float v, bool on) {
                  "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v))), "r"((uint32_t)on)
                  : "memory");
 }
+__device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, bool on) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.shared::cluster.f32 [%0], %1;\n\t}" ::"r"(addr), "f"(v), "r"((uint32_t)on) : "memory");
+}
 __device__ __forceinline__ void store4(float* p, const float4& v) { __stcs(reinterpret_cast<float4*>(p), v); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float4& v) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
@@ -120,7 +122,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
     const tc5::WaitCtx ctx{&sh->abort_flag, a.err};
     pdk_pdl_launch_dependents();
 
-    uint64_t acc[kPlanes][BN / 2u];
+    float acc[kPlanes][BN];
     bool ok = true;
     if (warp == 0) {
         // ------------------------------------------------------------ producer (whole warp, one lane issues)
@@ -183,7 +185,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
 #pragma unroll
         for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
-            for (uint32_t i = 0; i < BN / 2u; ++i) acc[p][i] = 0u;
+            for (uint32_t i = 0; i < BN; ++i) acc[p][i] = 0.0f;
         float next_x[BN / 32u], next_w[2] = {0.0f, 0.0f};
         auto fetch = [&](uint32_t kb) {
 #pragma unroll
@@ -206,26 +208,37 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_full[buf], bphase, ctx, tc5::kErrTmemFullWait, buf));
             if (!ok) break;
             tc5::fence_after_sync();
+            // two loads of 32 columns on their way, where a product of 128 columns leaves registers for that; plane p's columns are p * BN .. + BN - 1
+            constexpr uint32_t kLoads = C::kCols / 32u, kAtOnce = C::kCols <= 64u ? 2u : 1u;
+            uint32_t r[kAtOnce][32];
+            const uint32_t from = lanes + buf * C::kCols;
+            auto add = [&](uint32_t l) {
+                const float4* s = reinterpret_cast<const float4*>(turn + l * 32u);
 #pragma unroll
-            for (int p = 0; p < kPlanes; ++p)
-#pragma unroll
-                for (uint32_t c = 0; c < BN; c += 16u) {
-                    uint32_t r[16];
-                    tmem_ld_32x16(lanes + buf * C::kCols + p * BN + c, r);
-                    tc5::tmem_ld_wait();
-                    if (p == kPlanes - 1 && c + 16u == BN) {   // the last columns are in registers: the buffer goes back
-                        tc5::fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0u) tc5::mbar_arrive(&sh->acc_empty[buf]);
-                    }
-                    const ulonglong2* s = reinterpret_cast<const ulonglong2*>(turn + p * BN + c);
-#pragma unroll
-                    for (uint32_t i = 0; i < 4u; ++i) {
-                        const ulonglong2 s4 = s[i];
-                        fma2(acc[p][c / 2u + 2u * i], pack2(r[4u * i], r[4u * i + 1u]), s4.x);
-                        fma2(acc[p][c / 2u + 2u * i + 1u], pack2(r[4u * i + 2u], r[4u * i + 3u]), s4.y);
-                    }
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    const float4 s4 = s[i];
+                    float* to = acc[l * 32u / BN] + l * 32u % BN + 4u * i;
+                    const uint32_t(&v)[32] = r[l % kAtOnce];
+                    to[0] = fmaf(__uint_as_float(v[4u * i]), s4.x, to[0]);
+                    to[1] = fmaf(__uint_as_float(v[4u * i + 1u]), s4.y, to[1]);
+                    to[2] = fmaf(__uint_as_float(v[4u * i + 2u]), s4.z, to[2]);
+                    to[3] = fmaf(__uint_as_float(v[4u * i + 3u]), s4.w, to[3]);
                 }
+            };
+#pragma unroll
+            for (uint32_t l = 0; l < kLoads; l += kAtOnce) {
+#pragma unroll
+                for (uint32_t i = 0; i < kAtOnce && l + i < kLoads; ++i) tc5::tmem_ld_32x32(from + (l + i) * 32u, r[i]);
+#pragma unroll
+                for (uint32_t i = 0; i < kAtOnce && l + i < kLoads; ++i) tmem_ld_wait(r[i]);
+                if (l + kAtOnce >= kLoads) {   // the last columns are in registers: the buffer goes back
+                    tc5::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0u) tc5::mbar_arrive(&sh->acc_empty[buf]);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kAtOnce && l + i < kLoads; ++i) add(l + i);
+            }
             if (++buf == C::kBufs) { buf = 0; bphase ^= 1u; }
         }
     }
@@ -243,11 +256,8 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             const bool live = n0 + ch < a.out_dim;
             TO* out = y + (size_t)t0 * a.out_dim + n0 + ch;
 #pragma unroll
-            for (uint32_t i = 0; i < BN / 2u; ++i) {
-                const float2 v = unpack2(acc[0][i]);
-                store_if(out, v.x, live && 2u * i < n_tok);
-                out += a.out_dim;
-                store_if(out, v.y, live && 2u * i + 1u < n_tok);
+            for (uint32_t i = 0; i < BN; ++i) {
+                store_if(out, acc[0][i], live && i < n_tok);
                 out += a.out_dim;
             }
         }
@@ -262,11 +272,8 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
         if (warp >= 2u) {
             const uint32_t dst = cluster_addr(red, ch / cpr) + (rank * n_tok * cpr + ch % cpr) * 4u;
 #pragma unroll
-            for (uint32_t i = 0; i < BN / 2u; ++i) {
-                const float2 v = unpack2(acc[0][i]);
-                if (2u * i < n_tok) st_cluster(dst + 2u * i * cpr * 4u, v.x);
-                if (2u * i + 1u < n_tok) st_cluster(dst + (2u * i + 1u) * cpr * 4u, v.y);
-            }
+            for (uint32_t i = 0; i < BN; ++i)
+                st_cluster_if(dst + i * cpr * 4u, acc[0][i], i < n_tok);
         }
         cluster_sync();
         const uint32_t ch_lo = rank * cpr, groups = ch_lo < BM ? min(cpr, BM - ch_lo) / 4u : 0u;   // of four channels
@@ -294,19 +301,15 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
         const uint32_t tpr = (n_tok + split - 1u) / split;
         if (warp >= 2u) {
             const uint32_t own = (rank * 2u * tpr * BM + ch) * 4u;
-            uint32_t dst = 0u, owner = 0u, tok = tpr;
+            uint32_t owner = 0u, tok = 0u;
 #pragma unroll
-            for (uint32_t i = 0; i < BN; ++i) {
-                if (i < n_tok) {
-                    if (tok == tpr) {      // the first token of the next owner
-                        dst = cluster_addr(red, owner++) + own;
-                        tok = 0u;
-                    }
-                    const float2 g = unpack2(acc[0][i / 2u]), u = unpack2(acc[1][i / 2u]);
-                    st_cluster(dst + tok * BM * 4u, i & 1u ? g.y : g.x);
-                    st_cluster(dst + (tpr + tok) * BM * 4u, i & 1u ? u.y : u.x);
-                    ++tok;
-                }
+            for (uint32_t i = 0; i < BN; ++i) {      // no branches: one per token costs more than the stores
+                const uint32_t dst = cluster_addr(red, min(owner, split - 1u)) + own + tok * BM * 4u;
+                st_cluster_if(dst, acc[0][i], i < n_tok);
+                st_cluster_if(dst + tpr * BM * 4u, acc[kPlanes - 1][i], i < n_tok);
+                const bool next = ++tok == tpr;
+                owner += next ? 1u : 0u;
+                tok = next ? 0u : tok;
             }
         }
         if (split > 1u) cluster_sync();
@@ -335,24 +338,23 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
 }
 
 template <uint32_t BN, int kPlanes, typename TO>
-int launch_bn(const Call& c, cudaStream_t st) {
+int clusters(const uint32_t** resident) {
+    static PdkClusterCaps table;
+    return pdk_cluster_caps(table, (const void*)f8blk_split_kernel<BN, kPlanes, TO>, kThreads, Cfg<BN, kPlanes>::kSmemBytes, resident);
+}
+
+template <uint32_t BN, int kPlanes, typename TO>
+int launch_bn(const Call& c, uint32_t split, cudaStream_t st) {
     using C = Cfg<BN, kPlanes>;
     auto kern = f8blk_split_kernel<BN, kPlanes, TO>;
-    // How many clusters of s CTAs are resident at once.  The driver counts one CTA per SM for a kernel that allocates tensor memory;
-    // two run.
-    static PdkClusterCaps table;
     const uint32_t* resident = nullptr;
-    if (int rc = pdk_cluster_caps(table, (const void*)kern, kThreads, C::kSmemBytes, &resident)) return rc;
+    if (int rc = clusters<BN, kPlanes, TO>(&resident)) return rc;      // raises the kernel's shared memory limit on this device
     Args a{};
     a.ws0 = (const float*)c.ws[0]; a.ws1 = (const float*)c.ws[1]; a.xs = (const float*)c.xs; a.y = c.y; a.hs = (float*)c.hs;
     a.out_dim = c.out_dim; a.batch = c.batch; a.num_kb = blocks_of(c.in_dim);
     a.vec_store = (c.out_dim & 3u) == 0u && pdk_aligned(c.y, 4u * sizeof(TO)) ? 1u : 0u;
     a.err = pdk_error_word();
     const uint32_t tiles_t = c.batch / BN + (c.batch % BN != 0u), tiles_w = blocks_of(c.out_dim);
-    // the largest split whose clusters are all resident at once, of at least two blocks each
-    uint32_t split = a.num_kb / 2u < kPdkMaxCluster ? a.num_kb / 2u : kPdkMaxCluster;
-    while (split > 1u && (uint64_t)tiles_t * tiles_w > 2u * resident[split]) --split;
-    if (split == 0u) split = 1u;
 
     CUtensorMap tw0, tw1, tx;
     if (int rc = pdk_make_tmap_2d(&tw0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[0], c.in_dim, c.out_dim, c.in_dim, BK, BM)) return rc;
@@ -383,16 +385,20 @@ int launch_bn(const Call& c, cudaStream_t st) {
     return pdk_launch_status();
 }
 
-template <typename TO>
-int launch_gemm(const Call& c, cudaStream_t st) {
-    if (c.batch <= 32u) return launch_bn<32, 1, TO>(c, st);
-    if (c.batch <= 64u) return launch_bn<64, 1, TO>(c, st);
-    return launch_bn<128, 1, TO>(c, st);
+template <uint32_t BN>
+int launch_kind(const Call& c, int planes, bool bf16, uint32_t split, cudaStream_t st) {
+    if (planes == 2) return launch_bn<BN, 2, float>(c, split, st);
+    return bf16 ? launch_bn<BN, 1, __nv_bfloat16>(c, split, st) : launch_bn<BN, 1, float>(c, split, st);
 }
 
 }  // namespace
 
-int pdk_f8blk_split(const Call& c, int planes, bool bf16, cudaStream_t st) {
-    if (planes == 2) return c.batch <= 32u ? launch_bn<32, 2, float>(c, st) : launch_bn<64, 2, float>(c, st);
-    return bf16 ? launch_gemm<__nv_bfloat16>(c, st) : launch_gemm<float>(c, st);
+// resident[c]: how many clusters of s CTAs are resident at once with 32 << c tokens a tile.  0 or a cudaError_t.
+int pdk_f8blk_split_clusters(int planes, const uint32_t* resident[2]) {
+    if (int rc = planes == 2 ? clusters<32, 2, float>(&resident[0]) : clusters<32, 1, float>(&resident[0])) return rc;
+    return planes == 2 ? clusters<64, 2, float>(&resident[1]) : clusters<64, 1, float>(&resident[1]);
+}
+
+int pdk_f8blk_split(const Call& c, int planes, bool bf16, uint32_t cols, uint32_t split, cudaStream_t st) {
+    return cols == 32u ? launch_kind<32>(c, planes, bf16, split, st) : launch_kind<64>(c, planes, bf16, split, st);
 }

@@ -24,24 +24,7 @@ __device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const 
     return tc5::mbar_wait(bar, parity, ctx, code, detail);
 }
 
-// tensor memory -> registers: 32 lanes x 16 columns of 32 bits per warp
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-
 // The wait for this warp's loads, as what hands their registers on: nothing that uses them can be moved in front of it.
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
@@ -52,21 +35,6 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  : "memory");
 }
 
-// two f32 in one register pair, and acc += v * s on both: the roundings of two fused multiply-adds
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    uint32_t lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
-}
-
 // silu(g) * u.  The quotient is the hardware's (2 units, 0 where exp(-g) passes 2^126): an IEEE one has a rare path that is branched
 // to, which keeps neighbouring elements from overlapping.
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
@@ -74,5 +42,6 @@ __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 
 }  // namespace f8blk
 
 // f8blk_split.cu, f8blk_wide.cu: 0 or a cudaError_t
-int pdk_f8blk_split(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
-int pdk_f8blk_wide(const f8blk::Call& c, int planes, bool bf16, cudaStream_t st);
+int pdk_f8blk_split_clusters(int planes, const uint32_t* resident[2]);
+int pdk_f8blk_split(const f8blk::Call& c, int planes, bool bf16, uint32_t cols, uint32_t split, cudaStream_t st);
+int pdk_f8blk_wide(const f8blk::Call& c, int planes, bool bf16, uint32_t cols, cudaStream_t st);

@@ -6,7 +6,7 @@
 //
 //   warp 0      producer: a block of K of the tokens (16 KB) and of the channels (32 KB) per stage
 //   warp 1      MMA issuer: four MMAs per block into one of two buffers of 256 tensor-memory columns
-//   warps 2, 3  the scales: of 64 tokens each, times those of the two halves of the channels, into shared memory.  They arrive on the stage's
+//   warps 2, 3  the scales: of the tokens, times those of the two halves of the channels, into shared memory.  They arrive on the stage's
 //               barrier like the boxes, so whoever has a block's sums has its scales, without a wait of its own
 //   warps 4..11 the product: warp w has tokens 32 (w % 4) .. + 31 and 128 of the 256 columns, 128 registers a thread, and 64 more for columns on
 //               their way; the first four warps hand registers over for that
@@ -30,29 +30,44 @@ namespace {
 
 using namespace f8blk;
 
-constexpr uint32_t BM = 128, BN = 256, BNH = 128, BK = 128;   // tokens, channels, channels of a half, K per stage
-constexpr uint32_t kStages = 4;
-constexpr uint32_t kABytes = BM * BK, kBHalf = BNH * BK, kStageBytes = kABytes + 2u * kBHalf;
+constexpr uint32_t BM = 128, BK = 128;                        // tokens of a tile, K per stage
+constexpr uint32_t kABytes = BM * BK;
 constexpr uint32_t kWarps = 8, kFirst = 4;                    // that keep the product, and the first of them
 constexpr uint32_t kThreads = (kFirst + kWarps) * 32u;
 // registers a thread: 168 at launch (64,512 in all), 56 for the first four warps and 224 for the others after the split (64,512)
 constexpr uint32_t kRegsFew = 56, kRegsMany = 224;
 static_assert(kFirst * 32u * kRegsFew + kWarps * 32u * kRegsMany <= kThreads * 168u, "the split draws on what the launch has");
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kAhead = 4;                                // blocks whose scales a lane loads together
-// Scales are written when a stage is free and read when its sums are: at most the stages and the two buffers lie between.
-constexpr uint32_t kSlots = 8;
-static_assert(kStages + 2u <= kSlots, "a slot is written again after it was read");
+constexpr uint32_t kAhead = 2;                                // blocks whose scales a lane loads together
+constexpr uint32_t kSlots = 16;
 
+// BN columns of a tile: 256, or 128 where tiles of 256 would leave SMs without one
+template <uint32_t BN>
+struct Cfg {
+    static constexpr uint32_t kParts = BN / 128u;             // boxes of 128 channels, each with weight scales of its own
+    static constexpr uint32_t kStageBytes = kABytes + kParts * 128u * BK;
+    static constexpr uint32_t kStages = BN == 256u ? 4u : 6u;
+    static constexpr uint32_t kBufs = kTmemCols / BN;
+    static constexpr uint32_t kCols = BN / 2u;                // of a warp
+    // Warps that issue MMAs, alternate blocks each.  A block costs its issuer about 600 cycles of waits and issue: too many for 128 columns.
+    // With two buffers a second issuer's MMAs would only mix with the first's and finish both blocks late (359 us instead of 343).
+    static constexpr uint32_t kIssuers = BN == 256u ? 1u : 2u, kScalers = 3u - kIssuers, kRows = 4u / kScalers;   // and tokens a lane of the others
+    // scales are written when a stage is free and read when its sums are: at most the stages and the buffers lie between
+    static_assert(kStages + kBufs <= kSlots, "a slot is written again after it was read");
+    // a stage is summed again only after this buffer was handed back kBufs blocks later: the phase that is waited for cannot be missed
+    static_assert(kStages >= kBufs && kStages % kIssuers == 0u && kBufs % kIssuers == 0u, "an issuer keeps its own stages and buffers");
+};
+constexpr uint32_t kMaxStages = 6, kMaxBufs = 4;
+
+template <uint32_t kParts>
 struct Shared {
-    uint64_t full[kStages];
-    uint64_t empty[kStages];
-    uint64_t acc_full[2];
-    uint64_t acc_empty[2];
+    uint64_t full[kMaxStages];         // boxes and scales are there
+    uint64_t done[kMaxStages];         // the block is summed: its stage is free, its buffer full
+    uint64_t acc_empty[kMaxBufs];
     uint32_t tmem_base;
     int abort_flag;
     float amax[2][BM];
-    float scale[kSlots][2][BM];      // block % kSlots: the products of the scales, per half of the channels and token
+    float scale[kSlots][kParts][BM];   // block % kSlots: the products of the scales, per 128 channels and token
 };
 
 struct Args {
@@ -83,14 +98,14 @@ __device__ __forceinline__ uint4 piece(const float* v, __nv_bfloat16*) {
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// a thread's 128 channels of its token's row, `left` of which the row has
-template <typename TO>
-__device__ __forceinline__ void store_row(TO* out, const float (&v)[BNH], uint32_t left, uint32_t align) {
+// a thread's N channels of its token's row, `left` of which the row has
+template <uint32_t N, typename TO>
+__device__ __forceinline__ void store_row(TO* out, const float (&v)[N], uint32_t left, uint32_t align) {
     constexpr uint32_t kPer = 16u / sizeof(TO);
     if (align >= 16u) {       // rows end on a piece too
         const bool wide = align >= 32u;
 #pragma unroll
-        for (uint32_t i = 0; i < BNH; i += 2u * kPer) {
+        for (uint32_t i = 0; i < N; i += 2u * kPer) {
             const uint4 a = piece(v + i, out), b = piece(v + i + kPer, out);
             if (wide) {
                 if (i < left) store32(out + i, a, b);
@@ -101,33 +116,33 @@ __device__ __forceinline__ void store_row(TO* out, const float (&v)[BNH], uint32
         }
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < BNH; ++i)
+        for (uint32_t i = 0; i < N; ++i)
             if (i < left) put(out + i, v[i]);
     }
 }
 
-template <int kPlanes, typename TO>
+template <int kPlanes, uint32_t BN, typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
 f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w0,
                   const __grid_constant__ CUtensorMap tmap_w1, const Args a) {
+    using C = Cfg<BN>;
+    constexpr uint32_t kStages = C::kStages, kStageBytes = C::kStageBytes, kBufs = C::kBufs, kParts = C::kParts;
+    static_assert(kPlanes == 1 || BN == 256u, "a block of h has its 128 channels of gate and up in one tile");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
-    Shared* sh = reinterpret_cast<Shared*>(tiles + kStages * kStageBytes);
+    Shared<kParts>* sh = reinterpret_cast<Shared<kParts>*>(tiles + kStages * kStageBytes);
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    constexpr uint32_t kTileN = kPlanes == 2 ? BNH : BN;      // channels of y (of h) per tile
+    constexpr uint32_t kTileN = kPlanes == 2 ? 128u : BN;      // channels of y (of h) per tile
     const uint32_t tiles_m = (a.batch + BM - 1u) / BM, tiles_n = (a.out_dim + kTileN - 1u) / kTileN;
     const uint32_t n_tiles = tiles_m * tiles_n, w_blocks = (a.out_dim + 127u) / 128u;
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            tc5::mbar_init(&sh->full[s], 3);     // the expected-bytes arrival, two warps of scales
-            tc5::mbar_init(&sh->empty[s], 1);
+            tc5::mbar_init(&sh->full[s], 1u + C::kScalers);     // the expected-bytes arrival, the scales
+            tc5::mbar_init(&sh->done[s], 1);
         }
-        for (uint32_t b = 0; b < 2; ++b) {
-            tc5::mbar_init(&sh->acc_full[b], 1);
-            tc5::mbar_init(&sh->acc_empty[b], kWarps);
-        }
+        for (uint32_t b = 0; b < kBufs; ++b) tc5::mbar_init(&sh->acc_empty[b], kWarps);
         sh->abort_flag = 0;
         tc5::mbar_fence_init();
         tc5::tma_prefetch_desc(&tmap_x);
@@ -155,67 +170,83 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
             for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
                 const uint32_t m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * kTileN;
                 for (uint32_t kb = 0; kb < a.num_kb; ++kb) {
-                    ok = __all_sync(0xffffffffu, wait_soon(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, stage));
+                    ok = __all_sync(0xffffffffu, wait_soon(&sh->done[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, stage));
                     if (!ok) break;
                     uint8_t* s = tiles + stage * kStageBytes;
                     tc5::mbar_arrive_expect_tx_elect(&sh->full[stage], kStageBytes);
                     tc5::tma_load_2d_elect(s, &tmap_x, &sh->full[stage], (int32_t)(kb * BK), (int32_t)m0);
                     tc5::tma_load_2d_elect(s + kABytes, &tmap_w0, &sh->full[stage], (int32_t)(kb * BK), (int32_t)n0);
-                    tc5::tma_load_2d_elect(s + kABytes + kBHalf, kPlanes == 2 ? &tmap_w1 : &tmap_w0, &sh->full[stage], (int32_t)(kb * BK),
-                                           (int32_t)(kPlanes == 2 ? n0 : n0 + BNH));
+                    if (kParts == 2u)
+                        tc5::tma_load_2d_elect(s + kABytes + 128u * BK, kPlanes == 2 ? &tmap_w1 : &tmap_w0, &sh->full[stage], (int32_t)(kb * BK),
+                                               (int32_t)(kPlanes == 2 ? n0 : n0 + 128u));
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
             if (!ok && lane == 0)
                 for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies in flight still land in this CTA
             __syncwarp();
-        } else if (warp == 1u) {
-            // -------------------------------------------------------- MMA issuer (whole warp, one lane issues)
+        } else if (warp <= C::kIssuers) {
+            // -------------------------------------------------------- MMA issuers (whole warp, one lane issues)
             constexpr uint32_t idesc = tc5::idesc_f32acc(0u, 0u, BM, BN);
-            uint32_t stage = 0, phase = 0, block = 0;
-            for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x)
-                for (uint32_t kb = 0; kb < a.num_kb; ++kb, ++block) {
-                    const uint32_t buf = block & 1u, bphase = (block >> 1) & 1u;
-                    ok = __all_sync(0xffffffffu, wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage) &&
-                                                     wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf));
-                    if (!ok) break;
-                    tc5::fence_after_sync();
-                    const uint32_t a_addr = tc5::smem_u32(tiles + stage * kStageBytes);
-                    tc5::mma_f8f6f4_x4_elect(tmem_base + buf * BN, tc5::smem_desc_sw128(a_addr), tc5::smem_desc_sw128(a_addr + kABytes), idesc, 0u);
-                    tc5::mma_commit_elect(&sh->acc_full[buf]);
-                    tc5::mma_commit_elect(&sh->empty[stage]);
-                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
-                }
+            const uint32_t mine = warp - 1u, blocks = ((n_tiles - 1u - blockIdx.x) / gridDim.x + 1u) * a.num_kb;
+            uint32_t stage = mine, phase = 0, buf = mine, bphase = 0;
+            for (uint32_t block = mine; block < blocks && ok; block += C::kIssuers) {
+                const bool empty = wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf);
+                ok = __all_sync(0xffffffffu, wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage) && empty);
+                if (!ok) break;
+                tc5::fence_after_sync();
+                const uint32_t a_addr = tc5::smem_u32(tiles + stage * kStageBytes);
+                tc5::mma_f8f6f4_x4_elect(tmem_base + buf * BN, tc5::smem_desc_sw128(a_addr), tc5::smem_desc_sw128(a_addr + kABytes), idesc, 0u);
+                tc5::mma_commit_elect(&sh->done[stage]);
+                if ((stage += C::kIssuers) >= kStages) { stage = mine; phase ^= 1u; }
+                if ((buf += C::kIssuers) >= kBufs) { buf = mine; bphase ^= 1u; }
+            }
             pdk_pdl_wait();
         } else {
             // -------------------------------------------------------- scales
-            const uint32_t row = (warp - 2u) * 64u + lane;
+            constexpr uint32_t kRows = C::kRows;
+            const uint32_t row0 = (warp - 1u - C::kIssuers) * 32u * kRows + lane;
             uint32_t stage = 0, phase = 0, block = 0;
             pdk_pdl_wait();
             for (uint32_t tile = blockIdx.x; tile < n_tiles && ok; tile += gridDim.x) {
-                const uint32_t t = (tile % tiles_m) * BM + row, nb = (tile / tiles_m) * kTileN / 128u;
-                const float* x0 = a.xs + (size_t)min(t, a.batch - 1u) * a.num_kb;
-                const float* x1 = a.xs + (size_t)min(t + 32u, a.batch - 1u) * a.num_kb;
+                const uint32_t t = (tile % tiles_m) * BM + row0, nb = (tile / tiles_m) * kTileN / 128u;
+                const float* x[kRows];
+#pragma unroll
+                for (uint32_t i = 0; i < kRows; ++i) x[i] = a.xs + (size_t)min(t + 32u * i, a.batch - 1u) * a.num_kb;
                 const float* w0 = a.ws0 + (size_t)nb * a.num_kb;
-                const float* w1 = kPlanes == 2 ? a.ws1 + (size_t)nb * a.num_kb : a.ws0 + (size_t)min(nb + 1u, w_blocks - 1u) * a.num_kb;
-                for (uint32_t k0 = 0; k0 < a.num_kb && ok; k0 += kAhead) {
-                    float x[2][kAhead], w[2][kAhead];
+                const float* w1 = kPlanes == 2 ? a.ws1 + (size_t)nb * a.num_kb : a.ws0 + (size_t)min(nb + kParts - 1u, w_blocks - 1u) * a.num_kb;
+                float nx[kRows][kAhead], nw[kParts][kAhead];      // the next blocks', on their way while the last ones are handed on
+                auto fetch = [&](uint32_t k0) {
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; ++j) {
                         const uint32_t kb = min(k0 + j, a.num_kb - 1u);
-                        x[0][j] = x0[kb]; x[1][j] = x1[kb]; w[0][j] = w0[kb]; w[1][j] = w1[kb];
+#pragma unroll
+                        for (uint32_t i = 0; i < kRows; ++i) nx[i][j] = x[i][kb];
+                        nw[0][j] = w0[kb];
+                        if (kParts == 2u) nw[kParts - 1u][j] = w1[kb];
                     }
+                };
+                fetch(0u);
+                for (uint32_t k0 = 0; k0 < a.num_kb && ok; k0 += kAhead) {
+                    float cx[kRows][kAhead], cw[kParts][kAhead];
+#pragma unroll
+                    for (uint32_t j = 0; j < kAhead; ++j) {
+#pragma unroll
+                        for (uint32_t i = 0; i < kRows; ++i) cx[i][j] = nx[i][j];
+#pragma unroll
+                        for (uint32_t h = 0; h < kParts; ++h) cw[h][j] = nw[h][j];
+                    }
+                    fetch(k0 + kAhead);
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; ++j) {
                         if (k0 + j >= a.num_kb || !ok) break;
-                        ok = __all_sync(0xffffffffu, wait_soon(&sh->empty[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, 16u + stage));
+                        ok = __all_sync(0xffffffffu, wait_soon(&sh->done[stage], phase ^ 1u, ctx, tc5::kErrEmptyWait, 16u + stage));
                         if (!ok) break;
-                        float(&slot)[2][BM] = sh->scale[block++ % kSlots];
+                        float(&slot)[kParts][BM] = sh->scale[block++ % kSlots];
 #pragma unroll
-                        for (uint32_t h = 0; h < 2u; ++h) {
-                            slot[h][row] = x[0][j] * w[h][j];
-                            slot[h][row + 32u] = x[1][j] * w[h][j];
-                        }
+                        for (uint32_t h = 0; h < kParts; ++h)
+#pragma unroll
+                            for (uint32_t i = 0; i < kRows; ++i) slot[h][row0 + 32u * i] = cx[i][j] * cw[h][j];
                         __syncwarp();
                         if (lane == 0u) tc5::mbar_arrive(&sh->full[stage]);
                         if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -228,25 +259,26 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         // ------------------------------------------------------------ the product
         const uint32_t quarter = warp & 3u, half = (warp - kFirst) >> 2;
         const uint32_t row = quarter * 32u + lane;           // token of the tile
-        // columns: 128 in a row, or 64 of gate's and the same of up's
-        const uint32_t lanes = tmem_base + ((quarter * 32u) << 16) + half * (kPlanes == 2 ? 64u : BNH);
-        constexpr uint32_t kSecond = kPlanes == 2 ? BNH : 64u;                // where the second 64 start
+        // columns: half of the tile's in a row, or 64 of gate's and the same of up's
+        constexpr uint32_t kCols = C::kCols, kSecond = kPlanes == 2 ? 128u : 64u;    // and where the second 64 start
+        const uint32_t lanes = tmem_base + ((quarter * 32u) << 16) + half * (kPlanes == 2 ? 64u : kCols);
         uint32_t block = 0;
         bool ok = true;
         pdk_pdl_wait();
         for (uint32_t tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
             const uint32_t m0 = (tile % tiles_m) * BM, n0 = (tile / tiles_m) * kTileN;
             const uint32_t t = m0 + row;
-            float acc[BNH];
+            float acc[kCols];
 #pragma unroll
-            for (uint32_t i = 0; i < BNH; ++i) acc[i] = 0.0f;
+            for (uint32_t i = 0; i < kCols; ++i) acc[i] = 0.0f;
             for (uint32_t kb = 0; kb < a.num_kb && ok; ++kb, ++block) {
-                const uint32_t buf = block & 1u, bphase = (block >> 1) & 1u;
-                ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_full[buf], bphase, ctx, tc5::kErrTmemFullWait, buf));
+                const uint32_t buf = block % kBufs, stage = block % kStages;
+                ok = __all_sync(0xffffffffu, wait_soon(&sh->done[stage], block / kStages & 1u, ctx, tc5::kErrTmemFullWait, stage));
                 if (!ok) break;
-                const float s0 = sh->scale[block % kSlots][kPlanes == 2 ? 0u : half][row], s1 = kPlanes == 2 ? sh->scale[block % kSlots][1][row] : s0;
                 tc5::fence_after_sync();
-                // two loads on their way at a time; the second pair follows the first into its registers
+                const float(&slot)[kParts][BM] = sh->scale[block % kSlots];
+                const float s0 = slot[kPlanes == 2 || kParts == 1u ? 0u : half][row], s1 = kPlanes == 2 ? slot[kParts - 1u][row] : s0;
+                // two loads on their way at a time; a second pair follows the first into its registers
                 uint32_t r[2][32];
                 const uint32_t from = lanes + buf * BN;
                 auto add = [&](uint32_t c) {
@@ -257,20 +289,22 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                 tc5::tmem_ld_32x32(from + 32u, r[1]);
                 tmem_ld_wait(r[0]);
                 tmem_ld_wait(r[1]);
-                add(0u);
-                tc5::tmem_ld_32x32(from + kSecond, r[0]);
-                add(1u);
-                tc5::tmem_ld_32x32(from + kSecond + 32u, r[1]);
-                tmem_ld_wait(r[0]);
-                tmem_ld_wait(r[1]);
+                if constexpr (kCols == 128u) {
+                    add(0u);
+                    tc5::tmem_ld_32x32(from + kSecond, r[0]);
+                    add(1u);
+                    tc5::tmem_ld_32x32(from + kSecond + 32u, r[1]);
+                    tmem_ld_wait(r[0]);
+                    tmem_ld_wait(r[1]);
+                }
                 tc5::fence_before_sync();      // every column is in registers: the buffer goes back
                 __syncwarp();
                 if (lane == 0u) tc5::mbar_arrive(&sh->acc_empty[buf]);
-                add(2u);
-                add(3u);
+                add(kCols / 32u - 2u);
+                add(kCols / 32u - 1u);
             }
             if constexpr (kPlanes == 1) {
-                const uint32_t n = n0 + half * BNH;
+                const uint32_t n = n0 + half * kCols;
                 if (ok && t < a.batch && n < a.out_dim)
                     store_row(reinterpret_cast<TO*>(a.y) + (size_t)t * a.out_dim + n, acc, a.out_dim - n, a.row_align);
             } else {
@@ -308,25 +342,25 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     }
 }
 
-template <int kPlanes, typename TO>
+template <int kPlanes, uint32_t BN, typename TO>
 int launch_wide(const Call& c, cudaStream_t st) {
     CUtensorMap tx, tw0, tw1;
     if (int rc = pdk_make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.xq, c.in_dim, c.batch, c.in_dim, BK, BM)) return rc;
-    if (int rc = pdk_make_tmap_2d(&tw0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[0], c.in_dim, c.out_dim, c.in_dim, BK, BNH)) return rc;
+    if (int rc = pdk_make_tmap_2d(&tw0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[0], c.in_dim, c.out_dim, c.in_dim, BK, 128u)) return rc;
     tw1 = tw0;
     if (kPlanes == 2)
-        if (int rc = pdk_make_tmap_2d(&tw1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[1], c.in_dim, c.out_dim, c.in_dim, BK, BNH)) return rc;
+        if (int rc = pdk_make_tmap_2d(&tw1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.w[1], c.in_dim, c.out_dim, c.in_dim, BK, 128u)) return rc;
     Args a{};
     a.ws0 = (const float*)c.ws[0]; a.ws1 = (const float*)c.ws[1]; a.xs = (const float*)c.xs; a.y = c.y; a.hs = (float*)c.hs;
     a.out_dim = c.out_dim; a.batch = c.batch; a.num_kb = blocks_of(c.in_dim);
     const uint64_t where = (uint64_t)(uintptr_t)c.y | (uint64_t)c.out_dim * sizeof(TO);
     a.row_align = where % 32u == 0u ? 32u : where % 16u == 0u ? 16u : (uint32_t)sizeof(TO);
     a.err = pdk_error_word();
-    const size_t smem = (size_t)kStages * kStageBytes + sizeof(Shared) + 1024u;
-    auto kern = f8blk_wide_kernel<kPlanes, TO>;
+    const size_t smem = (size_t)Cfg<BN>::kStages * Cfg<BN>::kStageBytes + sizeof(Shared<Cfg<BN>::kParts>) + 1024u;
+    auto kern = f8blk_wide_kernel<kPlanes, BN, TO>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    const uint32_t tile_n = kPlanes == 2 ? BNH : BN;
+    const uint32_t tile_n = kPlanes == 2 ? 128u : BN;
     const uint64_t n_tiles = (uint64_t)((c.batch + BM - 1u) / BM) * ((c.out_dim + tile_n - 1u) / tile_n);
     if (n_tiles > 0x7fffffffull) return cudaErrorInvalidValue;
     const uint32_t sms = (uint32_t)pdk_sm_count();
@@ -335,7 +369,8 @@ int launch_wide(const Call& c, cudaStream_t st) {
 
 }  // namespace
 
-int pdk_f8blk_wide(const Call& c, int planes, bool bf16, cudaStream_t st) {
-    if (planes == 2) return launch_wide<2, float>(c, st);
-    return bf16 ? launch_wide<1, __nv_bfloat16>(c, st) : launch_wide<1, float>(c, st);
+int pdk_f8blk_wide(const Call& c, int planes, bool bf16, uint32_t cols, cudaStream_t st) {
+    if (planes == 2) return launch_wide<2, 256, float>(c, st);
+    if (cols == 128u) return bf16 ? launch_wide<1, 128, __nv_bfloat16>(c, st) : launch_wide<1, 128, float>(c, st);
+    return bf16 ? launch_wide<1, 256, __nv_bfloat16>(c, st) : launch_wide<1, 256, float>(c, st);
 }

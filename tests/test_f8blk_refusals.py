@@ -71,6 +71,13 @@ def test_gate_up_refuses_rows_that_the_down_projection_could_not_read(ff):
     assert status("pdk_f8blk_gate_up", *[A] * 8, 128, ff, 4) == INVALID
 
 
+def test_plan_query_refuses_what_is_no_product():
+    lib, plan = C.CDLL(pb.lib_path()), (C.c_uint32 * 3)()
+    for args in ((0, 128, 128, 1), (3, 128, 128, 1), (1, 0, 128, 1), (1, 128, 0, 1), (1, 128, 128, 0)):
+        assert lib.pdk_f8blk_plan(*args, plan) == INVALID
+    assert lib.pdk_f8blk_plan(1, 128, 128, 1, None) == INVALID
+
+
 def test_quantizers_refuse_more_blocks_than_their_numbers_hold():
     for name in ("pdk_quantize_e4m3_blk", "pdk_quantize_e4m3_blk_bf16", "pdk_bf16_to_f8blk", "pdk_f8blk_dequant"):
         assert status(name, A, A, A, 0xFFFFFFFC, 0xFFFFFFFF) == INVALID

@@ -1,6 +1,8 @@
 """e4m3 with a scale per block of 128 on a GPU.  The quantizers, the weight loader and the way back are held to the rule's exact bits; the
 products to an f64 product of the same codes and scales, within what f32 sums of that length can be off; the gated front to its f64
 value within that and half a step of its e4m3 result."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -225,7 +227,9 @@ class Operands:
 
 SHAPES = [(1, 1, 16), (1, 128, 128), (3, 5, 48), (2, 1024, 5120), (7, 129, 144), (17, 1000, 400), (31, 300, 17408), (33, 257, 2048),
           (64, 640, 1040), (65, 384, 512), (100, 5000, 640), (130, 260, 272), (200, 1024, 1024), (300, 700, 4000), (513, 1280, 256),
-          (257, 19000, 128), (1000, 4900, 400), (1100, 2600, 1536)]
+          (257, 19000, 128), (1000, 4900, 400), (1100, 2600, 1536),
+          # the plans that these do not take: 64 tokens a tile, whole and split; 256 channels a tile, several rounds, rows off 16 bytes
+          (33, 48, 16), (3000, 48, 2400), (140, 14192, 288), (2000, 4900, 1040), (1100, 2602, 1536)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -292,9 +296,24 @@ def check_gate_up(o, hq, hs):
     assert (off <= np.maximum(half_step(v), half_step(np.abs(v) + slack)) + slack).all()
 
 
-@pytest.mark.parametrize("m,ff,k", [(1, 16, 16), (1, 128, 128), (2, 2880, 2880), (7, 144, 144), (17, 1008, 400), (33, 272, 2048), (64, 640, 1040),
-                                    (65, 384, 512), (130, 272, 272), (200, 1024, 1024), (300, 704, 4000), (257, 9600, 128), (1000, 4912, 400),
-                                    (1100, 2608, 1536)])
+GATED = [(1, 16, 16), (1, 128, 128), (2, 2880, 2880), (7, 144, 144), (17, 1008, 400), (33, 272, 2048), (64, 640, 1040),
+         (65, 384, 512), (130, 272, 272), (200, 1024, 1024), (300, 704, 4000), (257, 9600, 128), (1000, 4912, 400),
+         (1100, 2608, 1536), (302, 2064, 7472)]
+
+
+def test_shapes_reach_every_plan(pack):
+    """What the product tests run: each kernel, each tile size of it, with and without a split of K."""
+    reached = {1: set(), 2: set()}
+    for planes, shapes in ((1, SHAPES), (2, GATED)):
+        for m, n, k in shapes:
+            plan = (ctypes.c_uint32 * 3)()
+            assert pack._lib.pdk_f8blk_plan(planes, k, n, m, plan) == 0
+            reached[planes].add((plan[0], plan[1], plan[2] > 1))
+    assert reached[1] == {(1, 32, False), (1, 32, True), (1, 64, False), (1, 64, True), (2, 128, False), (2, 256, False)}
+    assert reached[2] == {(1, 32, False), (1, 32, True), (1, 64, True), (2, 256, False)}
+
+
+@pytest.mark.parametrize("m,ff,k", GATED)
 def test_f8blk_gate_up(pack, m, ff, k):
     o = Operands(m, ff, k, 860 + m + ff + k, planes=2)
     hq, q_kept = guarded(m * ff, torch.uint8)
