@@ -205,27 +205,36 @@ __device__ __forceinline__ float block_max(float a, float* per_warp) {
     return m;
 }
 
-// A CTA per tile: 16 threads of 16 bytes span a tile's row, eight rows a thread, all its loads in flight before the maximum.
-__global__ void __launch_bounds__(kTileThreads) bf16_to_f8blk_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict__ q,
-                                                                     float* __restrict__ scale, uint32_t in_dim, uint32_t out_dim,
-                                                                     uint32_t per_row) {
+// A CTA per tile: 16 threads of 16 bytes span a tile's row, eight rows a thread, all its loads in flight before the maximum.  Four CTAs an
+// SM: 5120 x 17408 43 us, 6.2 TB/s (50 with the 87 registers a thread that the compiler would take, which leave room for two).
+__global__ void __launch_bounds__(kTileThreads, 4) bf16_to_f8blk_kernel(const __nv_bfloat16* __restrict__ w, uint8_t* __restrict__ q,
+                                                                        float* __restrict__ scale, uint32_t in_dim, uint32_t out_dim,
+                                                                        uint32_t per_row) {
     __shared__ float per_warp[kTileThreads / 32u];
     const uint32_t tile_n = blockIdx.x / per_row, tile_k = blockIdx.x - tile_n * per_row;
     const uint32_t col = tile_k * kBlock + (threadIdx.x & 15u) * 8u, row0 = tile_n * kBlock + (threadIdx.x >> 4);
+    // this thread's rows of the tile, 16 apart
+    const uint32_t rows = col < in_dim && row0 < out_dim ? (min(out_dim - row0, kBlock - (threadIdx.x >> 4)) + 15u) / 16u : 0u;
+    const size_t at = (size_t)row0 * in_dim + col, step = (size_t)in_dim * 16u;
     Piece<__nv_bfloat16> piece[8];
+    const __nv_bfloat16* from = w + at;
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i) {
         piece[i].zero();
-        if (col < in_dim && row0 + 16u * i < out_dim) piece[i].load(w + (size_t)(row0 + 16u * i) * in_dim + col);
+        if (i < rows) piece[i].load(from);
+        from += step;
     }
     float a = 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i) a = fmaxf(a, piece[i].amax());
     const float s = scale_of(block_max(a, per_warp)), r = 1.0f / s;
     if (threadIdx.x == 0u) scale[blockIdx.x] = s;
+    uint8_t* to = q + at;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i)
-        if (col < in_dim && row0 + 16u * i < out_dim) piece[i].store(q + (size_t)(row0 + 16u * i) * in_dim + col, r);
+    for (uint32_t i = 0; i < 8u; ++i) {
+        if (i < rows) piece[i].store(to, r);
+        to += step;
+    }
 }
 
 // Any row length and alignment, element by element: the tile is read twice.
