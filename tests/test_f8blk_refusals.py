@@ -81,6 +81,8 @@ def test_plan_query_refuses_what_is_no_product():
 def test_quantizers_refuse_more_blocks_than_their_numbers_hold():
     for name in ("pdk_quantize_e4m3_blk", "pdk_quantize_e4m3_blk_bf16", "pdk_bf16_to_f8blk", "pdk_f8blk_dequant"):
         assert status(name, A, A, A, 0xFFFFFFFC, 0xFFFFFFFF) == INVALID
+        assert status(name, A, A, A, 0xFFFFFF80, 1) == INVALID           # a row whose last block's end has no number
+    assert status("pdk_bf16_to_f8blk", A, A, A, 1, 0xFFFFFF80) == INVALID
 
 
 def test_add_rmsnorm_quant_refusals():

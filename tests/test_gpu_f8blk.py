@@ -262,6 +262,19 @@ def test_f8blk_gemm_into_rows_off_a_16_byte_boundary(pack, m, n, k, t):
     assert torch.equal(got[0], got[1])
 
 
+def test_f8blk_gemm_of_more_than_32_bits_of_results(pack):
+    """Rows of y behind 2^32 elements."""
+    m, n, k = 65700, 65600, 128
+    o = Operands(m, n, k, 845)
+    y = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    pack.call("pdk_f8blk_gemm_bf16", o.w[0][0], o.w[0][1], o.xq, o.xs, y, k, n, m)
+    assert pack.device_error() == 0
+    for rows in (slice(0, 3), slice(m - 130, m)):
+        ref, ab = o.x64[rows] @ o.w[0][2].T, o.x64[rows].abs() @ o.w[0][2].abs().T
+        tol = (2 * B + 1 + 10) * ULP * ab * (1 + 2.0 ** -8) + 2.0 ** -8 * ref.abs()
+        assert bool(((y[rows].double() - ref).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 256, 512), (50, 384, 640), (700, 2304, 512)])
 def test_f8blk_gemm_keeps_nan_in_its_row_and_column(pack, m, n, k):
     o = Operands(m, n, k, 840)
