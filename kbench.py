@@ -4,6 +4,7 @@ the memory-bound operators (operand clones rotated so consecutive launches
 never touch the same bytes), one JSON line per case.
 
     python kbench.py --op f8row_gemm --m 4096 --n 17408 --k 5120
+    python kbench.py --op f8blk_gate_up --m 1            # block-scaled FP8; f8blk_gemm is the product
     python kbench.py --op q4k_gemv --m 1
     python kbench.py --op q8_gemv
     python kbench.py --op f8row_gemm --out f32 --pack /path/to/another-pack.so
@@ -251,6 +252,37 @@ def bench_f8(ex, a):
     err = rel_err(y.view(m, n)[:toks, :rows], xd @ wd.t())
     return sec, {"bound": "tensor", "flops": 2.0 * m * n * k, "parity_rel_l2": err,
                  "parity_ok": err < (5e-3 if a.out == "bf16" else 1e-4)}
+
+
+def bench_f8blk(ex, a):
+    """Block-scaled e4m3: the product, or with --op f8blk_gate_up the gated front."""
+    m, n, k, gated = a.m, a.n, a.k, a.op == "f8blk_gate_up"
+    blocks = lambda v: (v + 127) // 128  # noqa: E731
+    planes = [[ex.bf16_to_f8blk(synth.normal(n * k, 11 + i, 0.02, "cuda").to(torch.bfloat16), k, n) for i in range(1 + gated)]
+              for _ in range(clones_for((1 + gated) * n * k) if m <= 512 else 1)]
+    x = synth.normal(m * k, 5, 1.0, "cuda")
+    xq, xs = torch.zeros(m * k, dtype=torch.uint8, device="cuda"), torch.zeros(m * blocks(k), device="cuda")
+    ex.quantize_e4m3_blk(x, xq, xs, k, m)
+    wide = lambda q, s, rows, r: q.view(-1, k)[:rows].view(torch.float8_e4m3fn).float() * (  # noqa: E731
+        s.view(-1, blocks(k)).repeat_interleave(128, 1)[:, :k].repeat_interleave(r, 0)[:rows])
+    if gated:
+        hq, hs = torch.zeros(m * n, dtype=torch.uint8, device="cuda"), torch.zeros(m * blocks(n), device="cuda")
+        call = lambda i: ex.f8blk_gate_up(*planes[i % len(planes)], xq, xs, hq, hs, m)  # noqa: E731
+    else:
+        y = torch.zeros(m * n, dtype=torch.bfloat16 if a.out == "bf16" else torch.float32, device="cuda")
+        call = lambda i: ex.f8blk_gemm(planes[i % len(planes)][0], xq, xs, y, m)  # noqa: E731
+    sec = time_launches(call, a.iters)
+    # spot check: a corner against an f32 product of the decoded operands
+    rows, toks = min(n, 384), min(m, 96)
+    p = [wide(xq, xs, toks, 1) @ wide(w.data, w.scale, rows, 128).t() for w in planes[0]]
+    if gated:
+        got = hq.view(m, n)[:toks, :rows].view(torch.float8_e4m3fn).float() * hs.view(m, -1)[:toks].repeat_interleave(128, 1)[:, :rows]
+        err, most = rel_err(got, p[0] * torch.sigmoid(p[0]) * p[1]), 4e-2       # an e4m3 result
+    else:
+        err, most = rel_err(y.view(m, n)[:toks, :rows], p[0]), 5e-3 if a.out == "bf16" else 1e-4
+    return sec, {"bound": "both", "flops": 2.0 * m * n * k * (1 + gated),
+                 "bytes": (1 + gated) * n * k + m * k + m * n * (1 if gated else 2 if a.out == "bf16" else 4), "parity_rel_l2": err,
+                 "parity_ok": err < most}
 
 
 def bench_nvf4(ex, a):
@@ -649,8 +681,8 @@ def bench_moe_nvf4(ex, a):
     return sec, {"bound": "hbm", "bytes": int(distinct * per_expert + T * embd * 2 * 2), "distinct_experts": distinct}
 
 
-OPS = {"tc5_probe": bench_tc5_probe, "f8_shard": bench_f8_shard, "norm_nvf4": bench_norm_nvf4, "q4k_w4a8": bench_q4k_w4a8, "nvf4_gemv": bench_nvf4_gemv, "moe_nvf4": bench_moe_nvf4, "moe_ep": bench_moe_ep, "moe_mxfp4": bench_moe, "nvf4_gemm": bench_nvf4, "q4k_gemv": bench_q4k, "q8_gemv": bench_q8, "f8row_gemm": bench_f8}
-DEFAULTS = {"tc5_probe": (0, 0, 0), "f8_shard": (4096, 27648, 5120), "norm_nvf4": (64, 0, 5120), "q4k_w4a8": (4, 25600, 5120), "nvf4_gemv": (1, 17408, 5120), "moe_nvf4": (64, 2880, 2880), "moe_ep": (64, 2880, 2880), "moe_mxfp4": (64, 2880, 2880), "nvf4_gemm": (8192, 17408, 5120), "q4k_gemv": (1, 25600, 5120), "q8_gemv": (1, 17408, 5120), "f8row_gemm": (4096, 17408, 5120)}
+OPS = {"f8blk_gemm": bench_f8blk, "f8blk_gate_up": bench_f8blk, "tc5_probe": bench_tc5_probe, "f8_shard": bench_f8_shard, "norm_nvf4": bench_norm_nvf4, "q4k_w4a8": bench_q4k_w4a8, "nvf4_gemv": bench_nvf4_gemv, "moe_nvf4": bench_moe_nvf4, "moe_ep": bench_moe_ep, "moe_mxfp4": bench_moe, "nvf4_gemm": bench_nvf4, "q4k_gemv": bench_q4k, "q8_gemv": bench_q8, "f8row_gemm": bench_f8}
+DEFAULTS = {"f8blk_gemm": (4096, 17408, 5120), "f8blk_gate_up": (2048, 17408, 5120), "tc5_probe": (0, 0, 0), "f8_shard": (4096, 27648, 5120), "norm_nvf4": (64, 0, 5120), "q4k_w4a8": (4, 25600, 5120), "nvf4_gemv": (1, 17408, 5120), "moe_nvf4": (64, 2880, 2880), "moe_ep": (64, 2880, 2880), "moe_mxfp4": (64, 2880, 2880), "nvf4_gemm": (8192, 17408, 5120), "q4k_gemv": (1, 25600, 5120), "q8_gemv": (1, 17408, 5120), "f8row_gemm": (4096, 17408, 5120)}
 
 
 class Case:

@@ -14,14 +14,18 @@
 // Gated front: the first 128 channels of a tile are gate's, the others up's beside them.  A warp's columns are then 64 of gate's and the
 // same 64 of up's, so a thread gates its own sums; only the maximum of a token's block crosses to the other half's warp.
 //
-// What bounds it (cycles per block of a tile; 4096 tokens, 5120 x 17408): the tensor core needs 514, loads and additions from
-// tensor memory by themselves 357, the two with their hand-over 630 with operands in place, boxes from L2 (48 KB) 730 without the additions;
-// all together 830, 343 us, 2.1 PFLOP/s.  On the way there:
+// Tiles of 128 channels, four buffers of 128 columns and half the columns a warp, where tiles of 256 would leave SMs without one: 200 tokens
+// through 5120 x 5120 14.4 us instead of 22.0.
+//
+// What bounds it (cycles per block of a 256-channel tile, 512 tokens through 17408 x 9472, one tile per SM): the tensor core needs 514, loads from
+// tensor memory and additions by themselves 357, both with their hand-over 630 with operands in place, the boxes from L2 (48 KB) 730
+// without the additions; all together 851.  4096 tokens through 5120 x 17408: 350 us in short runs (2.1 PFLOP/s), about 400 in long ones, where
+// the power limit takes the clock to 1.4 GHz.  Measured on the way there:
 //   scales read from global memory by the eight warps, 32 sectors a load              +330 cycles
 //   brought by warps 2 and 3, but under barriers of their own                         +170
-//   packed multiply-adds (fma.rn.f32x2): the pairs are moved together first           +200
-//   pairs of SMs (cta_group::2, two thirds of the L2 traffic): every block crosses between the SMs twice, and the barriers of two CTAs in
-//   lock step cost what the traffic saves: 377 us at best
+//   packed multiply-adds (fma.rn.f32x2): their pairs are moved together first         +200
+//   a block's loads started in front of the last block's additions                    +100
+//   pairs of SMs (cta_group::2, two thirds of the L2 traffic)                         +140 to +250: every block crosses between the SMs twice
 // Every wait is bounded; a role that gives up goes on through the loop without waiting or touching memory, so that the named
 // barriers of the others meet.
 #include "f8blk_tc5.cuh"
