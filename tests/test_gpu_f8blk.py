@@ -140,13 +140,27 @@ def test_quantize_blk_nan_and_infinity(pack, t, k):
     assert np.array_equal(v[[0, 1, 3]], v_ref)
 
 
+def test_quantize_blk_into_codes_off_a_boundary(pack):
+    rows, k = 5, 384
+    x = wild(rows, k, 725)
+    s_ref, v_ref = rule(x, 1)
+    for before in (16, 17, 18):
+        q, kept = guarded(rows * k, torch.uint8, before)
+        s = torch.zeros(rows * blocks(k), dtype=torch.float32, device="cuda")
+        pack.call("pdk_quantize_e4m3_blk", dev_f32(x.reshape(-1)), q, s, k, rows)
+        torch.cuda.synchronize()
+        assert np.array_equal(s.cpu().numpy().reshape(rows, -1), s_ref) and kept()
+        assert np.array_equal(e4m3_value(q.cpu().numpy()).reshape(rows, k), v_ref)
+
+
 @pytest.mark.parametrize("n,k", [(1, 16), (128, 128), (129, 144), (37, 640), (300, 1000), (260, 130), (5, 7)])
-def test_bf16_to_f8blk_and_back_bit_exact(pack, n, k):
+@pytest.mark.parametrize("before", [16, 17])
+def test_bf16_to_f8blk_and_back_bit_exact(pack, n, k, before):
     w = torch.from_numpy(wild(n, k, 730 + n + k)).to(torch.bfloat16)
     ref = w.float().numpy()
-    q, q_kept = guarded(n * k, torch.uint8)
+    q, q_kept = guarded(n * k, torch.uint8, before)
     s, s_kept = guarded(blocks(n) * blocks(k), torch.float32)
-    y, y_kept = guarded(n * k, torch.float32)
+    y, y_kept = guarded(n * k, torch.float32, before)
     pack.call("pdk_bf16_to_f8blk", w.cuda(), q, s, k, n)
     pack.call("pdk_f8blk_dequant", q, s, y, k, n)
     torch.cuda.synchronize()
@@ -406,15 +420,25 @@ def test_ffn_forward_eager_captured_and_on_another_stream(pack):
     assert pack.device_error() == 0
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 1024, 5120), (300, 700, 2000)])
+@pytest.mark.parametrize("m,n,k", [(5, 1024, 5120), (300, 700, 2000), (302, 2064, 7472), (700, 2304, 512), (1100, 2608, 1536)])
 def test_f8blk_products_repeat_their_bits(pack, m, n, k):
-    """Split sums meet in a fixed order: repeated calls give the same bits."""
-    o = Operands(m, n, k, 890)
-    y = [torch.zeros(m, n, device="cuda") for _ in range(4)]
-    for t in y:
-        pack.call("pdk_f8blk_gemm", o.w[0][0], o.w[0][1], o.xq, o.xs, t, k, n, m)
+    """Sums are added in a fixed order: calls repeated on two streams at once give the same bits."""
+    o = Operands(m, n, k, 890, planes=2)
+    (g, gs, _), (u, us, _) = o.w
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    torch.cuda.synchronize()
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 2]):
+            y, hq, hs = torch.zeros(m, n, device="cuda"), torch.zeros(m, n, dtype=torch.uint8, device="cuda"), torch.zeros(m, blocks(n), device="cuda")
+            st = streams[i % 2].cuda_stream
+            pack.call("pdk_f8blk_gemm", g, gs, o.xq, o.xs, y, k, n, m, stream=st)
+            if n % 16 == 0:
+                pack.call("pdk_f8blk_gate_up", g, gs, u, us, o.xq, o.xs, hq, hs, k, n, m, stream=st)
+            outs.append((y, hq, hs))
     assert pack.device_error() == 0
-    assert all(torch.equal(t, y[0]) for t in y[1:])
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
 
 
 def test_f8blk_through_the_operator_layer():
