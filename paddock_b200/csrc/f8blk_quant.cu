@@ -254,28 +254,33 @@ __global__ void __launch_bounds__(kTileThreads) bf16_to_f8blk_any_kernel(const _
         if (col < in_dim) q[(size_t)row * in_dim + col] = code1(__bfloat162float(w[(size_t)row * in_dim + col]), r);
 }
 
-// A CTA per tile, a warp per row of it: four codes a lane in, 16 bytes out, eight rows' loads in flight.
+// A CTA per tile, 16 lanes a row of it: eight codes a lane in, 32 bytes out, eight rows' loads in flight.  One store of 32 bytes rather than
+// two of 16 (`whole`: y is on a 32-byte boundary): 5120 x 5003 21.2 us, 6.05 TB/s, instead of 22.3.
 __global__ void __launch_bounds__(kTileThreads) f8blk_dequant_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale,
-                                                                     float* __restrict__ y, uint32_t in_dim, uint32_t out_dim, uint32_t per_row) {
+                                                                     float* __restrict__ y, uint32_t in_dim, uint32_t out_dim, uint32_t per_row,
+                                                                     uint32_t whole) {
     const uint32_t tile_n = blockIdx.x / per_row, tile_k = blockIdx.x - tile_n * per_row;
-    const uint32_t col = tile_k * kBlock + (threadIdx.x & 31u) * 4u, row0 = tile_n * kBlock + (threadIdx.x >> 5);
+    const uint32_t col = tile_k * kBlock + (threadIdx.x & 15u) * 8u, row0 = tile_n * kBlock + (threadIdx.x >> 4);
     pdk_pdl_launch_dependents();
     pdk_pdl_wait();
     const float s = scale[blockIdx.x];
+    const uint32_t rows = col < in_dim && row0 < out_dim ? (min(out_dim - row0, kBlock - (threadIdx.x >> 4)) + 15u) / 16u : 0u;
+    const size_t at = (size_t)row0 * in_dim + col, step = (size_t)in_dim * 16u;
+    uint2 c[8];
 #pragma unroll
-    for (uint32_t half = 0; half < 2u; ++half) {
-        uint32_t c[8];
+    for (uint32_t i = 0; i < 8u; ++i) c[i] = i < rows ? *reinterpret_cast<const uint2*>(q + at + i * step) : make_uint2(0u, 0u);
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t row = row0 + (half * 8u + i) * 8u;
-            c[i] = col < in_dim && row < out_dim ? __ldcs(reinterpret_cast<const uint32_t*>(q + (size_t)row * in_dim + col)) : 0u;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t row = row0 + (half * 8u + i) * 8u;
-            const float2 a = values2(c[i] & 0xffffu), b = values2(c[i] >> 16);
-            if (col < in_dim && row < out_dim)
-                __stcs(reinterpret_cast<float4*>(y + (size_t)row * in_dim + col), make_float4(a.x * s, a.y * s, b.x * s, b.y * s));
+    for (uint32_t i = 0; i < 8u; ++i) {
+        const float2 v0 = values2(c[i].x & 0xffffu), v1 = values2(c[i].x >> 16), v2 = values2(c[i].y & 0xffffu), v3 = values2(c[i].y >> 16);
+        if (i >= rows) continue;
+        float* p = y + at + i * step;
+        if (whole) {
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v0.x * s), "f"(v0.y * s), "f"(v1.x * s), "f"(v1.y * s),
+                         "f"(v2.x * s), "f"(v2.y * s), "f"(v3.x * s), "f"(v3.y * s)
+                         : "memory");
+        } else {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v0.x * s, v0.y * s, v1.x * s, v1.y * s);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v2.x * s, v2.y * s, v3.x * s, v3.y * s);
         }
     }
 }
@@ -348,7 +353,9 @@ PDK_EXPORT int pdk_f8blk_dequant(const void* data, const void* scale, void* y, u
     if (in_dim == 0u || out_dim == 0u) return 0;
     if (!plane_ok(data, 1, scale, y, 4, in_dim, out_dim)) return cudaErrorInvalidValue;
     const uint32_t per_row = f8blk::blocks_of(in_dim), tiles = per_row * f8blk::blocks_of(out_dim);
-    auto kern = (in_dim & 3u) == 0u && pdk_aligned(data, 4) && pdk_aligned(y, 16) ? f8blk_dequant_kernel : f8blk_dequant_any_kernel;
-    return pdk_launch_pdl(kern, dim3(tiles), dim3(kTileThreads), 0, (cudaStream_t)stream, (const uint8_t*)data, (const float*)scale, (float*)y,
-                          in_dim, out_dim, per_row);
+    if ((in_dim & 7u) == 0u && pdk_aligned(data, 8) && pdk_aligned(y, 16))
+        return pdk_launch_pdl(f8blk_dequant_kernel, dim3(tiles), dim3(kTileThreads), 0, (cudaStream_t)stream, (const uint8_t*)data, (const float*)scale,
+                              (float*)y, in_dim, out_dim, per_row, pdk_aligned(y, 32) ? 1u : 0u);
+    return pdk_launch_pdl(f8blk_dequant_any_kernel, dim3(tiles), dim3(kTileThreads), 0, (cudaStream_t)stream, (const uint8_t*)data, (const float*)scale,
+                          (float*)y, in_dim, out_dim, per_row);
 }

@@ -154,7 +154,7 @@ def test_quantize_blk_into_codes_off_a_boundary(pack):
 
 
 @pytest.mark.parametrize("n,k", [(1, 16), (128, 128), (129, 144), (37, 640), (300, 1000), (260, 130), (5, 7)])
-@pytest.mark.parametrize("before", [16, 17])
+@pytest.mark.parametrize("before", [16, 17, 20])          # y on a 32-byte, a 4-byte and a 16-byte boundary
 def test_bf16_to_f8blk_and_back_bit_exact(pack, n, k, before):
     w = torch.from_numpy(wild(n, k, 730 + n + k)).to(torch.bfloat16)
     ref = w.float().numpy()
