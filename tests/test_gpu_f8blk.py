@@ -243,7 +243,8 @@ SHAPES = [(1, 1, 16), (1, 128, 128), (3, 5, 48), (2, 1024, 5120), (7, 129, 144),
           (64, 640, 1040), (65, 384, 512), (100, 5000, 640), (130, 260, 272), (200, 1024, 1024), (300, 700, 4000), (513, 1280, 256),
           (257, 19000, 128), (1000, 4900, 400), (1100, 2600, 1536),
           # the plans that these do not take: 64 tokens a tile, whole and split; 256 channels a tile, several rounds, rows off 16 bytes
-          (33, 48, 16), (3000, 48, 2400), (140, 14192, 288), (2000, 4900, 1040), (1100, 2602, 1536)]
+          # and more than 48 tiles of tokens, whose last group is not full
+          (6300, 2200, 144), (33, 48, 16), (3000, 48, 2400), (140, 14192, 288), (2000, 4900, 1040), (1100, 2602, 1536)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -325,7 +326,7 @@ def check_gate_up(o, hq, hs):
 
 GATED = [(1, 16, 16), (1, 128, 128), (2, 2880, 2880), (7, 144, 144), (17, 1008, 400), (33, 272, 2048), (64, 640, 1040),
          (65, 384, 512), (130, 272, 272), (200, 1024, 1024), (300, 704, 4000), (257, 9600, 128), (1000, 4912, 400),
-         (1100, 2608, 1536), (302, 2064, 7472)]
+         (1100, 2608, 1536), (302, 2064, 7472), (6300, 1104, 144)]
 
 
 def test_shapes_reach_every_plan(pack):
