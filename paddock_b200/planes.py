@@ -137,10 +137,11 @@ class F8BlkPlane:
 
 
 class F8BlkFfnWorkspace:
-    """Buffers of one gated feed-forward block over F8BlkPlanes, for up to `tokens` tokens (allocated once, reused)."""
+    """Buffers of one gated feed-forward block over F8BlkPlanes, for up to `tokens` tokens of layers up to `embd` and `ff` wide
+    (allocated once, reused)."""
 
     def __init__(self, ex, embd, ff, tokens):
-        self.tokens = tokens
+        self.embd, self.ff, self.tokens = embd, ff, tokens
         self.xq = torch.empty(tokens * embd, dtype=torch.uint8, device=ex.device)
         self.xs = torch.empty(tokens * _blocks(embd), dtype=torch.float32, device=ex.device)
         self.hq = torch.empty(tokens * ff, dtype=torch.uint8, device=ex.device)
@@ -150,9 +151,11 @@ class F8BlkFfnWorkspace:
 def ffn_f8blk_forward(ex, gate, up, down, ws, x, proj, norm, eps, y, batch):
     """x += proj, then y = down(silu(gate(h)) * up(h)) of h = rmsnorm(x) * norm: residual add, norm and quantizer, the gated front,
     the down projection, one launch each.  y (f32 or bf16 [batch][embd]) is the next call's proj when it is f32."""
-    embd = gate.dims[0]
-    if down.dims != (gate.dims[1], embd):
+    embd, ff = gate.dims
+    if down.dims != (ff, embd):
         raise ValueError(f"down plane {down.dims} does not follow gate plane {gate.dims}")
+    if embd > ws.embd or ff > ws.ff:
+        raise ValueError(f"planes {gate.dims} in a workspace of {(ws.embd, ws.ff)}")
     if batch > ws.tokens:
         raise ValueError(f"{batch} tokens in a workspace of {ws.tokens}")
     ex.add_rmsnorm_quant_e4m3_blk(x, proj, norm, None, ws.xq, ws.xs, embd, eps, batch)

@@ -1,0 +1,62 @@
+"""What the feed-forward helper over block-scaled e4m3 planes refuses, on the host alone: a stub pack fails on any launch, so nothing may
+have been written when a call is refused."""
+import pytest
+import torch
+
+from paddock_b200 import planes as P
+
+EMBD, FF, TOKENS = 256, 512, 4
+
+
+class Refusing:
+    """A pack on which nothing may be launched."""
+    def call(self, name, *a, **k):
+        raise AssertionError(f"{name} launched")
+
+
+def executor(pack):
+    ex = P.GpuExecutor.__new__(P.GpuExecutor)
+    ex.pack, ex.device = pack, torch.device("cpu")
+    return ex
+
+
+def plane(in_dim, out_dim):
+    return P.F8BlkPlane(torch.zeros(in_dim * out_dim, dtype=torch.uint8), torch.zeros(P._blocks(in_dim) * P._blocks(out_dim)), (in_dim, out_dim))
+
+
+def forward(pack, monkeypatch, embd=EMBD, ff=FF, batch=TOKENS, **change):
+    """One call of the helper whose operands fit, but for what `change` replaces."""
+    monkeypatch.setattr(P, "_stream", lambda: 0)
+    ex = executor(pack)
+    args = {"gate": plane(embd, ff), "up": plane(embd, ff), "down": plane(ff, embd), "ws": P.F8BlkFfnWorkspace(ex, embd, ff, TOKENS),
+            "x": torch.zeros(batch * embd), "proj": torch.zeros(batch * embd), "norm": torch.ones(embd), "eps": 1e-6,
+            "y": torch.zeros(batch, embd), "batch": batch, **change}
+    P.ffn_f8blk_forward(ex, **args)
+
+
+class Counting:
+    def __init__(self):
+        self.names = []
+
+    def call(self, name, *a, **k):
+        self.names.append(name)
+
+
+def test_what_fits_is_three_launches(monkeypatch):
+    for y in (torch.zeros(TOKENS, EMBD), torch.zeros(TOKENS, EMBD, dtype=torch.bfloat16)):
+        pack = Counting()
+        forward(pack, monkeypatch, y=y)
+        assert pack.names == ["pdk_add_rmsnorm_quant_e4m3_blk", "pdk_f8blk_gate_up", "pdk_f8blk_gemm" + ("" if y.dtype == torch.float32 else "_bf16")]
+
+
+@pytest.mark.parametrize("embd,ff,tokens", [(EMBD - 128, FF, TOKENS), (EMBD, FF - 128, TOKENS), (EMBD - 16, FF, TOKENS), (EMBD, FF, TOKENS - 1),
+                                            (FF, EMBD, TOKENS)])
+def test_a_workspace_of_narrower_layers_is_refused(monkeypatch, embd, ff, tokens):
+    with pytest.raises(ValueError):
+        forward(Refusing(), monkeypatch, ws=P.F8BlkFfnWorkspace(executor(None), embd, ff, tokens))
+
+
+def test_a_workspace_of_wider_layers_is_taken(monkeypatch):
+    pack = Counting()
+    forward(pack, monkeypatch, ws=P.F8BlkFfnWorkspace(executor(None), EMBD + 128, FF + 16, TOKENS + 1))
+    assert len(pack.names) == 3
