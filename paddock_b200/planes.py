@@ -121,11 +121,12 @@ def _blocks(n):
 
 def _by_type(t, name):
     """The f32 or the bf16 form of a call."""
-    if t.dtype == torch.float32:
+    dtype = getattr(t, "dtype", None)
+    if dtype == torch.float32:
         return name
-    if t.dtype == torch.bfloat16:
+    if dtype == torch.bfloat16:
         return name + "_bf16"
-    raise TypeError(f"{name} takes f32 or bf16, not {t.dtype}")
+    raise TypeError(f"{name} takes f32 or bf16, not {dtype}")
 
 
 @dataclass
@@ -150,14 +151,23 @@ class F8BlkFfnWorkspace:
 
 def ffn_f8blk_forward(ex, gate, up, down, ws, x, proj, norm, eps, y, batch):
     """x += proj, then y = down(silu(gate(h)) * up(h)) of h = rmsnorm(x) * norm: residual add, norm and quantizer, the gated front,
-    the down projection, one launch each.  y (f32 or bf16 [batch][embd]) is the next call's proj when it is f32."""
+    the down projection, one launch each.  y (f32 or bf16 [batch][embd]) is the next call's proj when it is f32.  The first launch writes x,
+    so what a later one would refuse is refused here: a call that raises has left x as it was."""
     embd, ff = gate.dims
+    if up.dims != gate.dims:
+        raise ValueError(f"gate plane {gate.dims} and up plane {up.dims} differ")
     if down.dims != (ff, embd):
         raise ValueError(f"down plane {down.dims} does not follow gate plane {gate.dims}")
     if embd > ws.embd or ff > ws.ff:
         raise ValueError(f"planes {gate.dims} in a workspace of {(ws.embd, ws.ff)}")
     if batch > ws.tokens:
         raise ValueError(f"{batch} tokens in a workspace of {ws.tokens}")
+    if embd % 16 or ff % 16:
+        raise ValueError(f"planes {gate.dims}: rows of other than whole 16-byte pieces")
+    for plane in (gate, up, down):
+        if plane.data is None or plane.scale is None or plane.data.data_ptr() % 16:
+            raise ValueError("a plane's codes have to be there and start on a 16-byte boundary")
+    _by_type(y, "the result")
     ex.add_rmsnorm_quant_e4m3_blk(x, proj, norm, None, ws.xq, ws.xs, embd, eps, batch)
     ex.f8blk_gate_up(gate, up, ws.xq, ws.xs, ws.hq, ws.hs, batch)
     ex.f8blk_gemm(down, ws.hq, ws.hs, y, batch)

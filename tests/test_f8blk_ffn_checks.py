@@ -60,3 +60,35 @@ def test_a_workspace_of_wider_layers_is_taken(monkeypatch):
     pack = Counting()
     forward(pack, monkeypatch, ws=P.F8BlkFfnWorkspace(executor(None), EMBD + 128, FF + 16, TOKENS + 1))
     assert len(pack.names) == 3
+
+
+# ---- what a later launch of the three would refuse is refused before the first, which adds proj onto x
+def test_gate_and_up_of_different_sizes_are_refused_before_x_changes(monkeypatch):
+    for up in (plane(EMBD, FF + 128), plane(EMBD + 128, FF)):
+        with pytest.raises(ValueError):
+            forward(Refusing(), monkeypatch, up=up)
+
+
+@pytest.mark.parametrize("embd,ff", [(EMBD - 4, FF), (EMBD, FF - 8), (EMBD, FF - 1)])
+def test_widths_that_the_products_refuse_are_refused_before_x_changes(monkeypatch, embd, ff):
+    with pytest.raises(ValueError):
+        forward(Refusing(), monkeypatch, embd=embd, ff=ff)
+
+
+@pytest.mark.parametrize("y,error", [(torch.zeros(TOKENS, EMBD, dtype=torch.float16), TypeError), (torch.zeros(TOKENS, EMBD, dtype=torch.float64), TypeError),
+                                     (None, TypeError)])
+def test_a_result_that_the_down_projection_refuses_is_refused_before_x_changes(monkeypatch, y, error):
+    with pytest.raises(error):
+        forward(Refusing(), monkeypatch, y=y)
+
+
+@pytest.mark.parametrize("which", ["gate", "up", "down"])
+def test_planes_off_a_16_byte_boundary_are_refused_before_x_changes(monkeypatch, which):
+    dims = (FF, EMBD) if which == "down" else (EMBD, FF)
+    whole = torch.zeros(EMBD * FF + 32, dtype=torch.uint8)
+    off = (-whole.data_ptr()) % 16 + 8
+    off_boundary = P.F8BlkPlane(whole[off:off + EMBD * FF], torch.zeros(64), dims)
+    with pytest.raises(ValueError):
+        forward(Refusing(), monkeypatch, **{which: off_boundary})
+    with pytest.raises(ValueError):
+        forward(Refusing(), monkeypatch, **{which: P.F8BlkPlane(None, torch.zeros(64), dims)})
