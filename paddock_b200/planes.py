@@ -87,36 +87,51 @@ class GpuExecutor:
     # -- block-scaled e4m3 (no counterpart in the reference) -------------------------------
     def bf16_to_f8blk(self, w, in_dim, out_dim):
         """bf16 weights [out][in] on the device -> F8BlkPlane."""
+        _held_as(torch.bfloat16, w)
         data = torch.empty(out_dim * in_dim, dtype=torch.uint8, device=self.device)
         scale = torch.empty(_blocks(out_dim) * _blocks(in_dim), dtype=torch.float32, device=self.device)
         self.pack.call("pdk_bf16_to_f8blk", w, data, scale, in_dim, out_dim, stream=_stream())
         return F8BlkPlane(data, scale, (in_dim, out_dim))
 
     def f8blk_dequant(self, w, y):
+        _held_as(torch.float32, y)
         self.pack.call("pdk_f8blk_dequant", w.data, w.scale, y, w.dims[0], w.dims[1], stream=_stream())
 
     def quantize_e4m3_blk(self, x, q, scale, n, batch):
         """x f32 or bf16 [batch][n] -> codes and a scale per token and 128 elements."""
+        _held_as(torch.float32, scale)
         self.pack.call(_by_type(x, "pdk_quantize_e4m3_blk"), x, q, scale, n, batch, stream=_stream())
 
     def add_rmsnorm_quant_e4m3_blk(self, x, proj, w, xn, q, scale, n, eps, batch):
-        """x += proj (None: no residual); xn = rmsnorm(x) * w (None: not wanted); codes and scales of that."""
+        """x += proj (None: no residual); xn = rmsnorm(x) * w (None: not wanted); codes and scales of that.  All f32 but the codes."""
+        _held_as(torch.float32, x, proj, w, xn, scale)
         self.pack.call("pdk_add_rmsnorm_quant_e4m3_blk", x, proj, w, xn, q, scale, n, eps, batch, stream=_stream())
 
     def f8blk_gemm(self, w, xq, xs, y, batch):
         """y f32 or bf16 [batch][out]."""
+        _held_as(torch.float32, xs)
         self.pack.call(_by_type(y, "pdk_f8blk_gemm"), w.data, w.scale, xq, xs, y, w.dims[0], w.dims[1], batch, stream=_stream())
 
     def f8blk_gate_up(self, gate, up, xq, xs, hq, hs, batch):
         """Codes and scales of silu(x . Wg^T) * (x . Wu^T)."""
         if gate.dims != up.dims:
             raise ValueError(f"gate plane {gate.dims} and up plane {up.dims} differ")
+        _held_as(torch.float32, xs, hs)
         self.pack.call("pdk_f8blk_gate_up", gate.data, gate.scale, up.data, up.scale, xq, xs, hq, hs, gate.dims[0], gate.dims[1], batch,
                        stream=_stream())
 
 
 def _blocks(n):
     return -(-n // 128)
+
+
+def _held_as(dtype, *operands):
+    """The launches read and write elements of one size whatever they are given: a tensor of another floating type is refused.  None, addresses
+    and raw bytes pass."""
+    for t in operands:
+        dt = getattr(t, "dtype", None)
+        if dt is not None and dt is not dtype and dt.is_floating_point:
+            raise TypeError(f"an operand of {dtype} was expected, not of {dt}")
 
 
 def _by_type(t, name):

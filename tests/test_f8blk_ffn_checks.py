@@ -92,3 +92,61 @@ def test_planes_off_a_16_byte_boundary_are_refused_before_x_changes(monkeypatch,
         forward(Refusing(), monkeypatch, **{which: off_boundary})
     with pytest.raises(ValueError):
         forward(Refusing(), monkeypatch, **{which: P.F8BlkPlane(None, torch.zeros(64), dims)})
+
+
+# ---- types: the launches read f32 whatever floating type they are given, so a narrower tensor is read and written past its end
+NARROW = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("which", ["x", "proj", "norm"])
+@pytest.mark.parametrize("dtype", [*NARROW, torch.float64])
+def test_the_helper_refuses_a_residual_stream_of_other_types(monkeypatch, which, dtype):
+    with pytest.raises(TypeError):
+        forward(Refusing(), monkeypatch, **{which: torch.zeros(EMBD if which == "norm" else TOKENS * EMBD, dtype=dtype)})
+
+
+def test_the_residual_may_be_missing(monkeypatch):
+    pack = Counting()
+    forward(pack, monkeypatch, proj=None)
+    assert len(pack.names) == 3
+
+
+@pytest.mark.parametrize("dtype", [*NARROW, torch.float64])
+def test_f32_operands_of_the_single_calls_are_checked(monkeypatch, dtype):
+    monkeypatch.setattr(P, "_stream", lambda: 0)
+    ex, n, m = executor(Refusing()), 128, 2
+    bad, f32, codes, w = torch.zeros(m * n, dtype=dtype), torch.zeros(m * n), torch.zeros(m * n, dtype=torch.uint8), plane(n, m)
+    for i in (0, 1, 2, 3, 5):                                  # x, proj, w, xn, scale
+        args = [f32, f32, f32, f32, codes, f32]
+        args[i] = bad
+        with pytest.raises(TypeError):
+            ex.add_rmsnorm_quant_e4m3_blk(*args, n, 1e-6, m)
+    for call in (lambda: ex.f8blk_dequant(w, bad), lambda: ex.quantize_e4m3_blk(f32, codes, bad, n, m), lambda: ex.f8blk_gemm(w, codes, bad, f32, m),
+                 lambda: ex.f8blk_gate_up(w, w, codes, bad, codes, f32, m), lambda: ex.f8blk_gate_up(w, w, codes, f32, codes, bad, m)):
+        with pytest.raises(TypeError):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64])
+def test_weights_that_are_not_bf16_are_refused(monkeypatch, dtype):
+    monkeypatch.setattr(P, "_stream", lambda: 0)
+    with pytest.raises(TypeError):
+        executor(Refusing()).bf16_to_f8blk(torch.zeros(128 * 128, dtype=dtype), 128, 128)
+
+
+def test_what_may_be_missing_in_front_of_the_norm_may_still_be(monkeypatch):
+    monkeypatch.setattr(P, "_stream", lambda: 0)
+    pack = Counting()
+    executor(pack).add_rmsnorm_quant_e4m3_blk(torch.zeros(256), None, torch.ones(128), None, torch.zeros(256, dtype=torch.uint8), torch.zeros(2), 128, 1e-6, 2)
+    assert len(pack.names) == 1
+
+
+def test_addresses_and_raw_bytes_pass(monkeypatch):
+    """Operands without a floating type: an address, or a slice of a buffer of bytes."""
+    monkeypatch.setattr(P, "_stream", lambda: 0)
+    pack = Counting()
+    ex, raw = executor(pack), torch.zeros(1024, dtype=torch.uint8)
+    ex.add_rmsnorm_quant_e4m3_blk(raw.data_ptr(), raw, raw, None, raw, raw.data_ptr(), 128, 1e-6, 1)
+    ex.bf16_to_f8blk(raw, 64, 8)
+    ex.bf16_to_f8blk(raw.view(torch.int16), 64, 8)
+    assert len(pack.names) == 3
