@@ -188,8 +188,12 @@ class GpuExecutor:
         return self._plane(_lib().pdx_bf16_to_f8blk, p, C.c_uint64(in_dim), C.c_uint64(out_dim))
 
     def f8blk_upload(self, e4m3, scales, in_dim, out_dim):
+        """A checkpoint's codes and scales; scales as numbers (a bf16 tensor is widened first, its bits are no numbers)."""
         p, n, keep = _host(e4m3)
-        s = np.ascontiguousarray(scales, np.float32)
+        s = np.asarray(scales)
+        if s.dtype.kind != "f":
+            raise TypeError(f"f8blk_upload: scales are floating numbers, not {s.dtype}")
+        s = np.ascontiguousarray(s, np.float32)
         assert n == in_dim * out_dim and s.size == -(-out_dim // 128) * -(-in_dim // 128)
         return self._plane(_lib().pdx_f8blk_upload, p, s.ctypes.data_as(C.POINTER(C.c_float)), C.c_uint64(in_dim),
                            C.c_uint64(out_dim))
