@@ -55,6 +55,7 @@ struct Shared {
     uint64_t acc_empty[kMaxBufs];
     uint32_t tmem_base;
     int abort_flag;
+    int gave_up;      // some CTA of the cluster did not come to the end of its blocks
 };
 static_assert(sizeof(Shared) <= 256u, "control block");
 
@@ -79,6 +80,9 @@ __device__ __forceinline__ void store_if(__nv_bfloat16* p, float v, bool on) {
 }
 __device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, bool on) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q st.shared::cluster.f32 [%0], %1;\n\t}" ::"r"(addr), "f"(v), "r"((uint32_t)on) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void store4(float* p, const float4& v) { __stcs(reinterpret_cast<float4*>(p), v); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float4& v) {
@@ -109,6 +113,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             tc5::mbar_init(&sh->acc_empty[b], 4);
         }
         sh->abort_flag = 0;
+        sh->gave_up = 0;
         tc5::mbar_fence_init();
         tc5::tma_prefetch_desc(&tmap_w0);
         if (kPlanes == 2) tc5::tma_prefetch_desc(&tmap_w1);
@@ -251,11 +256,14 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
     if (split > 1u) cluster_sync();
     tc5::fence_after_sync();
     if (warp == 1) tc5::tmem_dealloc(tmem_base, C::kTmemCols);   // the last sums are in registers
+    // Where a wait ran out blocks of K are missing: with the partial products every CTA of the cluster hears of it, and none stores a result.
+    const bool gave_up = sh->abort_flag != 0;
+    if (gave_up && threadIdx.x < split) st_cluster_u32(cluster_addr(tc5::smem_u32(&sh->gave_up), threadIdx.x), 1u);
 
     const uint32_t ch = (warp & 3u) * 32u + lane;
     TO* y = reinterpret_cast<TO*>(a.y);
     if (kPlanes == 1 && split == 1u) {
-        if (warp >= 2u) {   // the tile is whole: 32 neighbouring channels per store
+        if (warp >= 2u && !gave_up) {   // the tile is whole: 32 neighbouring channels per store
             const bool live = n0 + ch < a.out_dim;
             TO* out = y + (size_t)t0 * a.out_dim + n0 + ch;
 #pragma unroll
@@ -279,6 +287,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
                 st_cluster_if(dst + i * cpr * 4u, acc[0][i], i < n_tok);
         }
         cluster_sync();
+        if (sh->gave_up) return;
         const uint32_t ch_lo = rank * cpr, groups = ch_lo < BM ? min(cpr, BM - ch_lo) / 4u : 0u;   // of four channels
         for (uint32_t i = threadIdx.x; i < groups * n_tok; i += kThreads) {
             const uint32_t tok = i / groups, g = (i - tok * groups) * 4u, n = n0 + ch_lo + g;
@@ -317,6 +326,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
         }
         if (split > 1u) cluster_sync();
         else __syncthreads();
+        if (sh->gave_up) return;
         const uint32_t tok_lo = rank * tpr, toks = tok_lo < n_tok ? min(tpr, n_tok - tok_lo) : 0u;
         const uint32_t n = n0 + lane * 4u, blocks = (a.out_dim + BM - 1u) / BM;
         for (uint32_t tok = warp; tok < toks; tok += kThreads / 32u) {
