@@ -333,11 +333,11 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                     acc[i] = gated(acc[i], acc[64u + i]);
                     m = fmaxf(m, fabsf(acc[i]));
                 }
-                sh->amax[half][row] = m;
+                sh->amax[half][row] = ok ? m : __int_as_float(0x7fffffff);       // NaN, which m never is: this half gave up
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float sc = scale_of(fmaxf(m, sh->amax[1u - half][row])), inv = 1.0f / sc;
+                const float other = sh->amax[1u - half][row], sc = scale_of(fmaxf(m, other)), inv = 1.0f / sc;
                 asm volatile("bar.sync 1, 256;" ::: "memory");       // read before the next tile's is written
-                if (ok && t < a.batch) {
+                if (ok && other == other && t < a.batch) {
                     const uint32_t n = n0 + half * 64u;
                     uint8_t* q = reinterpret_cast<uint8_t*>(a.y) + (size_t)t * a.out_dim + n;
 #pragma unroll

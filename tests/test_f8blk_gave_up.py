@@ -64,3 +64,11 @@ def test_the_whole_cluster_hears_of_a_wait_that_ran_out():
     assert zeroed < first < told < rest[0] and all(any(r < m.start() for r in rest) for m in re.finditer(r"if \(sh->gave_up", body)) and read > rest[0]
     tell = body[max(body.rfind(c, 0, told) for c in ";{}"):told]
     assert "gave_up && threadIdx.x < split" in tell and "const bool gave_up = sh->abort_flag != 0;" in body[first:told]
+
+
+def test_both_halves_of_a_token_hear_of_a_wait_that_ran_out():
+    """The gated front's scale is of both halves' warps: a half that gave up hands on NaN, and the other stores nothing either."""
+    body = kernel("f8blk_wide.cu")
+    handed = body.index("sh->amax[half][row] = ok ? m : __int_as_float(0x7fffffff);")
+    taken = body.index("other = sh->amax[1u - half][row]")
+    assert handed < body.index("bar.sync", handed) < taken < body.index("if (ok && other == other && t < a.batch)") < body.index("a.hs[")
