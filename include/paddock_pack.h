@@ -399,6 +399,9 @@ int pdk_tc5_issue_probe(uint32_t kind, uint32_t n_mma, void* cycles, void* strea
  * and the kernel returned normally, after which pdk_device_error() reads 0x507.  scratch = 4
  * bytes of device memory.  Synchronizes the stream. */
 int pdk_selftest_bounded_wait(uint32_t budget_us, void* scratch, void* stream);
+/* The same for the waits of the block-scaled e4m3 products, which try for a while before they look at the clock: one of two warps has
+ * the limit, the other leaves by its flag.  scratch 8 bytes; the error word then reads 5 << 8 | 8. */
+int pdk_selftest_f8blk_wait(uint32_t budget_us, void* scratch, void* stream);
 
 /* No counterpart in the reference.  Q4_K decode GEMV of one rank's row band whose epilogue stores
  * the band into every rank's full-length y over NVLink (y_ptrs: host array of n_ranks <= 8 device

@@ -34,6 +34,24 @@ int gemm(const void* w, const void* ws, const void* xq, const void* xs, void* y,
     return launch(c, 1, bf16, st);
 }
 
+// Two warps wait on barriers that nothing arrives on.  The first gives up after `budget_ns`, the second, whose own limit is the kernels', by the
+// first one's flag.  Each vote is the whole warp's, as behind every wait of the products.
+__global__ void wait_selftest_kernel(unsigned long long budget_ns, unsigned int* err_word, unsigned int* left) {
+    __shared__ uint64_t bar[2];
+    __shared__ int abort_flag;
+    const uint32_t warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        tc5::mbar_init(&bar[0], 1);
+        tc5::mbar_init(&bar[1], 1);
+        abort_flag = 0;
+        tc5::mbar_fence_init();
+    }
+    __syncthreads();
+    const tc5::WaitCtx ctx{&abort_flag, err_word};
+    const bool ok = __all_sync(0xffffffffu, f8blk::wait_soon(&bar[warp], 0u, ctx, tc5::kErrTestWait, 8u + warp, warp == 0u ? budget_ns : tc5::kWaitBudgetNs));
+    if ((threadIdx.x & 31u) == 0u) left[warp] = ok ? 2u : 1u;      // 1 = gave up as designed
+}
+
 }  // namespace
 
 PDK_EXPORT int pdk_f8blk_gemm(const void* data, const void* w_scale, const void* xq, const void* x_scale, void* y, uint32_t in_dim,
@@ -61,4 +79,18 @@ PDK_EXPORT int pdk_f8blk_plan(uint32_t planes, uint32_t in_dim, uint32_t out_dim
     if (int rc = plan_of((int)planes, in_dim, out_dim, batch, &p)) return rc;
     plan[0] = p.kernel; plan[1] = p.cols; plan[2] = p.split;
     return 0;
+}
+
+// Runs the timed-out path of these kernels' waits (one of two waits with a limit of budget_us, 1..100000): 0 when both gave up and the kernel
+// exited; pdk_device_error() then reads kErrTestWait << 8 | 8.  `scratch` is 8 bytes of device memory.  Synchronizes.
+PDK_EXPORT int pdk_selftest_f8blk_wait(uint32_t budget_us, void* scratch, void* stream) {
+    if (budget_us == 0u || budget_us > 100000u || !scratch || !pdk_aligned(scratch, 4)) return cudaErrorInvalidValue;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (cudaError_t e = cudaMemsetAsync(scratch, 0, 8, st); e != cudaSuccess) return (int)e;
+    wait_selftest_kernel<<<1, 64, 0, st>>>((unsigned long long)budget_us * 1000ull, pdk_error_word(), (unsigned int*)scratch);
+    if (int rc = pdk_launch_status()) return rc;
+    if (cudaError_t e = cudaStreamSynchronize(st); e != cudaSuccess) return (int)e;
+    unsigned int left[2] = {0u, 0u};
+    if (cudaError_t e = cudaMemcpy(left, scratch, 8, cudaMemcpyDeviceToHost); e != cudaSuccess) return (int)e;
+    return left[0] == 1u && left[1] == 1u ? 0 : cudaErrorUnknown;
 }

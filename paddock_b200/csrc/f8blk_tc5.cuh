@@ -18,10 +18,11 @@ struct Call {
 };
 
 // tc5::mbar_wait that reads the global timer only after some failed attempts: these waits are short and one per block of K.
-__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const tc5::WaitCtx& ctx, unsigned int code, unsigned int detail) {
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const tc5::WaitCtx& ctx, unsigned int code, unsigned int detail,
+                                          unsigned long long budget_ns = tc5::kWaitBudgetNs) {
     for (uint32_t i = 0; i < 64u; ++i)
         if (tc5::mbar_try_wait(bar, parity)) return true;
-    return tc5::mbar_wait(bar, parity, ctx, code, detail);
+    return tc5::mbar_wait(bar, parity, ctx, code, detail, budget_ns);
 }
 
 // The wait for this warp's loads, as what hands their registers on: nothing that uses them can be moved in front of it.

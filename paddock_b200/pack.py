@@ -139,6 +139,7 @@ _EXTRA_SIGS = {
     "pdk_peer_flags_wait": "puuu",
     "pdk_peer_flags_post": "ppuu",
     "pdk_selftest_bounded_wait": "up",
+    "pdk_selftest_f8blk_wait": "up",
     "pdk_tc5_issue_probe": "uup",
     "pdk_mxfp4_tc5_tile_scales": "pppuuu",
     "pdk_moe_prep_act_f4": "pppppppuuuuff",
