@@ -36,9 +36,10 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  : "memory");
 }
 
-// silu(g) * u.  The quotient is the hardware's (2 units, 0 where exp(-g) passes 2^126): an IEEE one has a rare path that is branched
-// to, which keeps neighbouring elements from overlapping.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
+// silu(g) * u, g / (1 + exp(-g)) * u.  The quotient is the hardware's (2 units): an IEEE one has a rare path that is branched to, which keeps
+// neighbouring elements from overlapping.  It is 0 for divisors beyond 2^126, so the divisor comes down by 4 and the quotient with it: both
+// are exact, a divisor that is a number stays below 2^126, and the quotient of no gate is below 2^-121 until exp(-g) is infinite.
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 0.25f * (1.0f + expf(-g))) * 0.25f * u; }
 
 }  // namespace f8blk
 
