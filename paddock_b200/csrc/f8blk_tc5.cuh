@@ -25,6 +25,11 @@ __device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const 
     return tc5::mbar_wait(bar, parity, ctx, code, detail, budget_ns);
 }
 
+// One arrival of a converged warp (tc5.cuh has why not from a branch of one lane).
+__device__ __forceinline__ void mbar_arrive_elect(uint64_t* bar) {
+    asm volatile(TC5_ELECT "@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(tc5::smem_u32(bar)) : "memory");
+}
+
 // The wait for this warp's loads, as what hands their registers on: nothing that uses them can be moved in front of it.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"

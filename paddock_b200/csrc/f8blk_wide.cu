@@ -7,7 +7,8 @@
 //   warp 0      producer: a block of K of the tokens (16 KB) and of the channels (32 KB) per stage
 //   warp 1      MMA issuer: four MMAs per block into one of two buffers of 256 tensor-memory columns
 //   warps 2, 3  the scales: of the tokens, times those of the two halves of the channels, into shared memory.  They arrive on the stage's
-//               barrier like the boxes, so whoever has a block's sums has its scales, without a wait of its own
+//               barrier like the boxes, so whoever has a block's sums has its scales, without a wait of its own: the issuer, which has waited
+//               for that barrier, arrives on the sums' one beside the tensor core, and its release hands the scales' stores on
 //   warps 4..11 the product: warp w has tokens 32 (w % 4) .. + 31 and 128 of the 256 columns, 128 registers a thread, and 64 more for columns on
 //               their way; the first four warps hand registers over for that
 //
@@ -156,7 +157,7 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
             tc5::mbar_init(&sh->full[s], 1u + C::kScalers);     // the expected-bytes arrival, the scales
-            tc5::mbar_init(&sh->done[s], 1);
+            tc5::mbar_init(&sh->done[s], 2);                    // the tensor core's arrival, the issuer's
         }
         for (uint32_t b = 0; b < kBufs; ++b) tc5::mbar_init(&sh->acc_empty[b], kWarps);
         sh->abort_flag = 0;
@@ -215,6 +216,7 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                 const uint32_t a_addr = tc5::smem_u32(tiles + stage * kStageBytes);
                 tc5::mma_f8f6f4_x4_elect(tmem_base + buf * BN, tc5::smem_desc_sw128(a_addr), tc5::smem_desc_sw128(a_addr + kABytes), idesc, 0u);
                 tc5::mma_commit_elect(&sh->done[stage]);
+                mbar_arrive_elect(&sh->done[stage]);
                 if ((stage += C::kIssuers) >= kStages) { stage = mine; phase ^= 1u; }
                 if ((buf += C::kIssuers) >= kBufs) { buf = mine; bphase ^= 1u; }
             }
