@@ -225,7 +225,7 @@ unsigned int pdk_device_error(void);
 /* ---- FP8 E4M3, one f32 scale per block of 128 ---------------------------------
  * No slots: the reference has no block-scaled e4m3 format.  The one of FP8 checkpoints that carry `weight_scale_inv`:
  *   weights      data e4m3 [out][in], scale f32 [ceil(out/128)][ceil(in/128)], one per 128 x 128 tile; w = code * scale.
- *                A checkpoint's two tensors are these planes byte for byte.
+ *                A checkpoint's two tensors are these planes byte for byte where its scales are f32 (bf16 ones are widened first).
  *   activations  q e4m3 [batch][in], scale f32 [batch][ceil(in/128)], one per token and 128 elements.
  * Quantizer of a block: a = max |v|, scale = max(a / 448, 2^-126), code = RN_e4m3(v * (1 / scale)), saturating, in f32.  A NaN or an
  * infinity makes every product of its token NaN. */
@@ -241,12 +241,15 @@ int pdk_add_rmsnorm_quant_e4m3_blk(void* x, const void* proj, const void* w, voi
 int pdk_bf16_to_f8blk(const void* bf16, void* data, void* scale, uint32_t in_dim, uint32_t out_dim, void* stream);
 int pdk_f8blk_dequant(const void* data, const void* scale, void* y, uint32_t in_dim, uint32_t out_dim, void* stream);
 /* y f32 / bf16 [batch][out] = sum over blocks b of x_scale[t][b] * w_scale[o/128][b] * (the block's product of codes), f32 sums.  Any
- * batch and out_dim; in_dim % 16 == 0, data and xq on 16-byte boundaries. */
+ * batch and out_dim; in_dim % 16 == 0, data and xq on 16-byte boundaries.  The two scales of a block are multiplied first, in f32: where
+ * that product is below 2^-126 it loses bits (all of them below 2^-150), and beyond f32 it is an infinity, NaN with a block whose
+ * codes come to 0, even where the whole term would be an ordinary number. */
 int pdk_f8blk_gemm(const void* data, const void* w_scale, const void* xq, const void* x_scale, void* y, uint32_t in_dim,
                    uint32_t out_dim, uint32_t batch, void* stream);
 int pdk_f8blk_gemm_bf16(const void* data, const void* w_scale, const void* xq, const void* x_scale, void* y, uint32_t in_dim,
                         uint32_t out_dim, uint32_t batch, void* stream);
-/* The front of a gated feed-forward block in one kernel: g, u = the products of two planes [ff][in]; h = g / (1 + exp(-g)) * u in f32,
+/* The front of a gated feed-forward block in one kernel: g, u = the products of two planes [ff][in]; h = g / (1 + exp(-g)) * u in f32
+ * (the exponential and the quotient to two units each; 0 from g = -88.73 on, where exp(-g) passes f32),
  * left quantized as the down projection reads it: hq e4m3 [batch][ff], h_scale f32 [batch][ceil(ff/128)].  in_dim % 16 == 0,
  * ff % 16 == 0; data, xq and hq on 16-byte boundaries. */
 int pdk_f8blk_gate_up(const void* gate_data, const void* gate_scale, const void* up_data, const void* up_scale, const void* xq,

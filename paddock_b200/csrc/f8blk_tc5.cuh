@@ -2,7 +2,8 @@
 //
 // The scales of a block are arbitrary f32, so the tensor core cannot apply them: it sums one 128-element block of K at a time into
 // tensor memory (kind::f8f6f4, f32), and the epilogue warps, which keep the product in registers, add it on with the block's
-// two scales while the tensor core does the next block.  That costs one fused multiply-add per element and block, and reading every
+// two scales while the tensor core does the next block.  The two are multiplied first, which is one number a token or column; a product of
+// theirs outside f32 takes the term with it, though the sum might have brought it back.  That costs one fused multiply-add per element and block, and reading every
 // element of tensor memory once per block.
 #pragma once
 #include "f8blk.cuh"

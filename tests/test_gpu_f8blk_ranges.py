@@ -51,3 +51,35 @@ def test_gated_unit_of_gates_down_to_where_the_exponential_overflows(pack, m, ff
     slack = (rel + 4 * ULP) * np.abs(want)
     off = np.abs(v - want)
     assert (off <= np.maximum(half_step(want), half_step(np.abs(want) + slack)) + slack)[whole].all()
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 272, 2048), (40, 400, 2048), (4000, 2064, 384), (300, 700, 256)])
+@pytest.mark.parametrize("xs,ws", [(2.0 ** -60, 2.0 ** -66), (2.0 ** -126, 1.0), (2.0 ** 100, 2.0 ** 9), (2.0 ** -100, 2.0 ** 120)])
+def test_products_under_scales_whose_product_f32_holds(pack, m, n, k, xs, ws):
+    """The two scales of a block are multiplied first.  Down to 2^-126 and up to where the result itself ends, with codes whose products and
+    sums are exact in f32, so is the result."""
+    g = torch.Generator(device="cuda").manual_seed(970)
+    code = lambda r: torch.tensor([0x00, ONE, TWO, MINUS_ONE], dtype=torch.uint8, device="cuda")[torch.randint(0, 4, (r, k), device="cuda", generator=g)]     # noqa: E731
+    xq, wq = code(m), code(n)
+    y = torch.zeros(m, n, device="cuda")
+    pack.call("pdk_f8blk_gemm", wq, torch.full((blocks(n), blocks(k)), ws, device="cuda"), xq, torch.full((m, blocks(k)), xs, device="cuda"), y, k, n, m)
+    assert pack.device_error() == 0
+    value = torch.tensor(e4m3_value(np.arange(256)), device="cuda")
+    want = (value[xq.long()] @ value[wq.long()].T) * xs * ws
+    assert torch.equal(y.double(), want)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 272, 2048), (4000, 2064, 128)])
+def test_products_under_scales_whose_product_passes_f32(pack, m, n, k):
+    """Beyond f32 the scales' product is an infinity: a sum of codes becomes one of its sign, a sum of zero NaN.  Below 2^-149 it is 0."""
+    xq, wq = torch.zeros(m, k, dtype=torch.uint8, device="cuda"), torch.zeros(n, k, dtype=torch.uint8, device="cuda")
+    xq[:, 0], wq[0::3, 0], wq[1::3, 0] = ONE, ONE, MINUS_ONE
+    y = torch.zeros(m, n, device="cuda")
+    big, small = (lambda r, s: torch.full((r, blocks(k)), s, device="cuda")), 2.0 ** -100
+    sx, sw = big(m, 1.0), big(blocks(n), 1.0)
+    sx[:, 0], sw[:, 0] = 2.0 ** 100, 2.0 ** 100
+    pack.call("pdk_f8blk_gemm", wq, sw, xq, sx, y, k, n, m)
+    assert bool((y[:, 0::3] == float("inf")).all()) and bool((y[:, 1::3] == float("-inf")).all()) and bool(y[:, 2::3].isnan().all())
+    sx[:, 0], sw[:, 0] = small, small
+    pack.call("pdk_f8blk_gemm", wq, sw, xq, sx, y, k, n, m)
+    assert pack.device_error() == 0 and bool((y == 0).all())
