@@ -54,6 +54,15 @@ def _ptr(a):
     return C.c_void_p(int(a))
 
 
+def _f32(a):
+    """Address of an f32 operand.  A tensor of a floating type of another size is refused: the launch would go past its end or between its
+    elements.  None, addresses and raw bytes pass."""
+    dt = getattr(a, "dtype", None)
+    if getattr(dt, "is_floating_point", False) and dt.itemsize != 4:
+        raise TypeError(f"an f32 operand was expected, not {dt}")
+    return _ptr(a)
+
+
 def _host(a):
     """(pointer, byte length, keep-alive) of host bytes."""
     arr = np.ascontiguousarray(a if isinstance(a, np.ndarray) else np.frombuffer(a, np.uint8))
@@ -242,20 +251,20 @@ class GpuExecutor:
         self._check(_lib().pdx_f8row_gemm(self._h, w._h, _ptr(xq), _ptr(xrs), _ptr(y), C.c_uint32(batch)))
 
     def quantize_e4m3_blk(self, x, q, scale, n, batch):
-        self._check(_lib().pdx_quantize_e4m3_blk(self._h, _ptr(x), _ptr(q), _ptr(scale), C.c_uint32(n), C.c_uint32(batch)))
+        self._check(_lib().pdx_quantize_e4m3_blk(self._h, _f32(x), _ptr(q), _f32(scale), C.c_uint32(n), C.c_uint32(batch)))
 
     def add_rmsnorm_quant_e4m3_blk(self, x, proj, w, xn, q, scale, n, eps, batch):
-        self._check(_lib().pdx_add_rmsnorm_quant_e4m3_blk(self._h, _ptr(x), _ptr(proj), _ptr(w), _ptr(xn), _ptr(q), _ptr(scale),
+        self._check(_lib().pdx_add_rmsnorm_quant_e4m3_blk(self._h, _f32(x), _f32(proj), _f32(w), _f32(xn), _ptr(q), _f32(scale),
                                                           C.c_uint32(n), C.c_float(eps), C.c_uint32(batch)))
 
     def f8blk_dequant(self, w, out):
-        self._check(_lib().pdx_f8blk_dequant(self._h, w._h, _ptr(out)))
+        self._check(_lib().pdx_f8blk_dequant(self._h, w._h, _f32(out)))
 
     def f8blk_gemm(self, w, xq, xs, y, batch):
-        self._check(_lib().pdx_f8blk_gemm(self._h, w._h, _ptr(xq), _ptr(xs), _ptr(y), C.c_uint32(batch)))
+        self._check(_lib().pdx_f8blk_gemm(self._h, w._h, _ptr(xq), _f32(xs), _f32(y), C.c_uint32(batch)))
 
     def f8blk_gate_up(self, gate, up, xq, xs, hq, hs, batch):
-        self._check(_lib().pdx_f8blk_gate_up(self._h, gate._h, up._h, _ptr(xq), _ptr(xs), _ptr(hq), _ptr(hs), C.c_uint32(batch)))
+        self._check(_lib().pdx_f8blk_gate_up(self._h, gate._h, up._h, _ptr(xq), _f32(xs), _ptr(hq), _f32(hs), C.c_uint32(batch)))
 
     def quantize_nvf4(self, x, q, scale, n):
         self._check(_lib().pdx_quantize_nvf4(self._h, _ptr(x), _ptr(q), _ptr(scale), C.c_uint32(n)))
