@@ -3,10 +3,12 @@
 // The estimates, us, were fitted to measured times of 100 random shapes (in 512 ... 17408, out 512 ... 17408, 1 ... 1500 tokens; gemm and gated
 // front) under every plan, cold weights.  The plan they pick takes 1.6 % longer than the best of the plans on average, 25 % at worst (3.3
 // against 4.1 us).  What they weigh:
-//   split   a CTA does its part of K alone and meets its cluster: 0.3 us a block of K of one plane, and 1.4 - 2 us and 25 ns a token for the
-//           meeting, which falls away where one CTA takes all of K.  Wins where a call has few tiles: 380 tokens, 13760 x 576 gated 21.9 us, wide 52.0
+//   split   a CTA does its part of K alone and meets its cluster.  One plane: 0.3 or 0.4 us a block of K, 0.2 more beside another CTA, and 1.7 or
+//           2.2 us and 25 ns a token for the meeting; where one CTA takes all of K, half of those 25 ns for the stores.  Gated: 0.5 or 1.0 us a block
+//           of both planes, 0.35 more beside another CTA, and 74 or 54 ns a token for the meeting, which is there with one CTA too.  Wins where a
+//           call has few tiles: 380 tokens, 13760 x 576 gated 25.9 us, wide 52.0
 //   wide    0.26 - 0.65 us a block of K and round of tiles.  Wins from the number of tiles on that fills the SMs: 648 tokens, 5888 x 2816 gated
-//           27.8 us, split 60.5; 128 channels a tile rather than 256 where those leave SMs empty: 200 tokens, 5120 x 5120 14.4 and 22.0
+//           27.3 us, split 60.3; 128 channels a tile rather than 256 where those leave SMs empty: 200 tokens, 5120 x 5120 15.2 and 22.2
 #pragma once
 #include <stdint.h>
 

@@ -16,7 +16,7 @@
 // same 64 of up's, so a thread gates its own sums; only the maximum of a token's block crosses to the other half's warp.
 //
 // Tiles of 128 channels, four buffers of 128 columns and half the columns a warp, where tiles of 256 would leave SMs without one: 200 tokens
-// through 5120 x 5120 14.4 us instead of 22.0.
+// through 5120 x 5120 15.2 us instead of 22.2.
 //
 // What bounds it (cycles per block of a 256-channel tile, 512 tokens through 17408 x 9472, one tile per SM): the tensor core needs 514, loads from
 // tensor memory and additions by themselves 357, both with their hand-over 630 with operands in place, the boxes from L2 (48 KB) 730
@@ -127,7 +127,7 @@ __device__ __forceinline__ void store_row(TO* out, const float (&v)[N], uint32_t
 }
 
 // Where tile number `tile` lies: token tiles fastest, so that a round of CTAs shares few of the weights and all of the tokens' rows in L2.  From
-// 49 token tiles on those are too many, and 32 at a time are gone through instead: 8192 tokens 8192 x 8192 536 -> 497 us, 5120 x 8192 342 -> 316.
+// 49 token tiles on those are too many, and 32 at a time are gone through instead: 8192 tokens 8192 x 8192 544 -> 505 us, 5120 x 8192 340 -> 333.
 // (Groups of 16, or weights fastest, are slower below that: 4096 tokens 5120 x 17408 354 and 425 us instead of 349.  The gated front gains
 // nothing from groups: 8192 tokens 5120 x 4096 340 us, without 336.)
 template <int kPlanes>

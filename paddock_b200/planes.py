@@ -154,7 +154,7 @@ class F8BlkPlane:
 
 class F8BlkFfnWorkspace:
     """Buffers of one gated feed-forward block over F8BlkPlanes, for up to `tokens` tokens of layers up to `embd` and `ff` wide
-    (allocated once, reused)."""
+    (allocated once, reused by calls that follow one another: one stream, or graphs replayed in turn)."""
 
     def __init__(self, ex, embd, ff, tokens):
         self.embd, self.ff, self.tokens = embd, ff, tokens
