@@ -166,6 +166,7 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (whole warp, one lane issues)
         uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
+        pdk_pdl_wait();   // the tokens come behind it: a limit that started earlier would count the launch in front
         for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
             ok = __all_sync(0xffffffffu, wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf) &&
                                              wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage));
@@ -181,7 +182,6 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
             if (++buf == C::kBufs) { buf = 0; bphase ^= 1u; }
         }
-        pdk_pdl_wait();
     } else {
         // ------------------------------------------------------------ a block's sums, scaled, onto the product
         pdk_pdl_wait();   // scales and y may still be in use by the previous kernel

@@ -208,6 +208,7 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
             constexpr uint32_t idesc = tc5::idesc_f32acc(0u, 0u, BM, BN);
             const uint32_t mine = warp - 1u, blocks = ((n_tiles - 1u - blockIdx.x) / gridDim.x + 1u) * a.num_kb;
             uint32_t stage = mine, phase = 0, buf = mine, bphase = 0;
+            pdk_pdl_wait();   // the boxes come behind it: a limit that started earlier would count the launch in front
             for (uint32_t block = mine; block < blocks && ok; block += C::kIssuers) {
                 const bool empty = wait_soon(&sh->acc_empty[buf], bphase ^ 1u, ctx, tc5::kErrTmemEmptyWait, buf);
                 ok = __all_sync(0xffffffffu, wait_soon(&sh->full[stage], phase, ctx, tc5::kErrFullWait, stage) && empty);
@@ -220,7 +221,6 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                 if ((stage += C::kIssuers) >= kStages) { stage = mine; phase ^= 1u; }
                 if ((buf += C::kIssuers) >= kBufs) { buf = mine; bphase ^= 1u; }
             }
-            pdk_pdl_wait();
         } else {
             // -------------------------------------------------------- scales
             constexpr uint32_t kRows = C::kRows;
