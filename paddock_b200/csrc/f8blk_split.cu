@@ -160,9 +160,6 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
             tc5::tma_load_2d_elect(smem + stage * C::kStageBytes + kPlanes * kABytes, &tmap_x, &sh->full[stage], (int32_t)(kb * BK), (int32_t)t0);
             if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
-        if (!ok && lane == 0)   // copies already issued still land in this CTA's shared memory
-            for (int i = 0; i < 64; ++i) __nanosleep(1000);
-        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (whole warp, one lane issues)
         uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
@@ -252,12 +249,13 @@ f8blk_split_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_con
     }
     tc5::fence_before_sync();
     __syncthreads();
+    const bool gave_up = sh->abort_flag != 0;
+    if (gave_up) wait_for_copies();
     // every CTA's stages are consumed from here on: they take the partial products
     if (split > 1u) cluster_sync();
     tc5::fence_after_sync();
     if (warp == 1) tc5::tmem_dealloc(tmem_base, C::kTmemCols);   // the last sums are in registers
     // Where a wait ran out blocks of K are missing: with the partial products every CTA of the cluster hears of it, and none stores a result.
-    const bool gave_up = sh->abort_flag != 0;
     if (gave_up && threadIdx.x < split) st_cluster_u32(cluster_addr(tc5::smem_u32(&sh->gave_up), threadIdx.x), 1u);
 
     const uint32_t ch = (warp & 3u) * 32u + lane;

@@ -31,6 +31,12 @@ __device__ __forceinline__ void mbar_arrive_elect(uint64_t* bar) {
     asm volatile(TC5_ELECT "@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(tc5::smem_u32(bar)) : "memory");
 }
 
+// For a CTA in which a wait ran out, every role past its loop: boxes that were requested, and MMAs that read them, may still be on their way
+// into memory that the next CTA gets.  64 us are far more than they take.
+__device__ __forceinline__ void wait_for_copies() {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+}
+
 // The wait for this warp's loads, as what hands their registers on: nothing that uses them can be moved in front of it.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"

@@ -200,9 +200,6 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
-            if (!ok && lane == 0)
-                for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies in flight still land in this CTA
-            __syncwarp();
         } else if (warp <= C::kIssuers) {
             // -------------------------------------------------------- MMA issuers (whole warp, one lane issues)
             constexpr uint32_t idesc = tc5::idesc_f32acc(0u, 0u, BM, BN);
@@ -357,6 +354,7 @@ f8blk_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 
     tc5::fence_before_sync();
     __syncthreads();
+    if (sh->abort_flag) wait_for_copies();
     if (warp == 1u) {
         tc5::fence_after_sync();
         tc5::tmem_dealloc(tmem_base, kTmemCols);

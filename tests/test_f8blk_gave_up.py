@@ -63,7 +63,7 @@ def test_the_whole_cluster_hears_of_a_wait_that_ran_out():
     read = body.index("if (sh->gave_up")
     assert zeroed < first < told < rest[0] and all(any(r < m.start() for r in rest) for m in re.finditer(r"if \(sh->gave_up", body)) and read > rest[0]
     tell = body[max(body.rfind(c, 0, told) for c in ";{}"):told]
-    assert "gave_up && threadIdx.x < split" in tell and "const bool gave_up = sh->abort_flag != 0;" in body[first:told]
+    assert "gave_up && threadIdx.x < split" in tell and "const bool gave_up = sh->abort_flag != 0;" in body[:told]
 
 
 def test_both_halves_of_a_token_hear_of_a_wait_that_ran_out():
@@ -72,3 +72,15 @@ def test_both_halves_of_a_token_hear_of_a_wait_that_ran_out():
     handed = body.index("sh->amax[half][row] = ok ? m : __int_as_float(0x7fffffff);")
     taken = body.index("other = sh->amax[1u - half][row]")
     assert handed < body.index("bar.sync", handed) < taken < body.index("if (ok && other == other && t < a.batch)") < body.index("a.hs[")
+
+
+@pytest.mark.parametrize("name", RESULTS)
+def test_a_cta_that_gave_up_stays_until_its_copies_have_landed(name):
+    """The role that gave up need not be the one with copies under way: the CTA waits, whoever it was, before it hands its shared memory on."""
+    body = kernel(name)
+    last = body.rindex("pdk_pdl_wait();")
+    met = body.index("__syncthreads();", last)
+    stays = re.search(r"if \(gave_up\) wait_for_copies\(\);|if \(sh->abort_flag\) wait_for_copies\(\);", body[met:])
+    assert stays and "cluster_sync" not in body[met:met + stays.start()] and "tmem_dealloc" not in body[met:met + stays.start()]
+    text = open(os.path.join(CSRC, "f8blk_tc5.cuh")).read()
+    assert re.search(r"void wait_for_copies\(\) \{\s*for \(int i = 0; i < 64; \+\+i\) __nanosleep\(1000\);", text)
