@@ -144,7 +144,8 @@ int pdx_rmsnorm_quant_e4m3_row(PdxExecutor* ex, const void* x, const void* w, vo
 int pdx_add_rmsnorm_scaled_quant_e4m3_row(PdxExecutor* ex, void* x, const void* proj, const void* w, void* xn, void* q,
                                           void* rs, uint32_t n, float eps, float pscale, uint32_t batch, int* fused);
 /* block-scaled e4m3 (paddock_pack.h has the formats): the activation quantizer, its form behind residual add and RMSNorm (proj and
- * xn may be NULL), the product (y f32) and the gated front (activations in f32; bf16 ones are calls of the pack) of a feed-forward block.  PDX_MISSING_OP on a pack without them. */
+ * xn may be NULL), the product and the gated front of a feed-forward block.  Activations and y are f32 (bf16: the pack's own calls).
+ * PDX_MISSING_OP on a pack without them. */
 int pdx_quantize_e4m3_blk(PdxExecutor* ex, const void* x, void* q, void* scale, uint32_t n, uint32_t batch);
 int pdx_add_rmsnorm_quant_e4m3_blk(PdxExecutor* ex, void* x, const void* proj, const void* w, void* xn, void* q, void* scale,
                                    uint32_t n, float eps, uint32_t batch);
