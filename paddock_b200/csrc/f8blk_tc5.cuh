@@ -49,9 +49,13 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
 }
 
 // silu(g) * u, g / (1 + exp(-g)) * u.  The quotient is the hardware's (2 units): an IEEE one has a rare path that is branched to, which keeps
-// neighbouring elements from overlapping.  It is 0 for divisors beyond 2^126, so the divisor comes down by 4 and the quotient with it: both
-// are exact, a divisor that is a number stays below 2^126, and the quotient of no gate is below 2^-121 until exp(-g) is infinite.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 0.25f * (1.0f + expf(-g))) * 0.25f * u; }
+// neighbouring elements from overlapping.  It is 0 for divisors beyond 2^126, which a negative gate has from -87.34 on: there the divisor comes
+// down by 4 and the quotient with it.  Both are exact, and a divisor that is a number stays below 2^126.  A positive gate's divisor is at most 2, and
+// its quotient would pass f32 for gates beyond 2^126.
+__device__ __forceinline__ float gated(float g, float u) {
+    const float c = g < 0.0f ? 0.25f : 1.0f;
+    return __fdividef(g, c * (1.0f + expf(-g))) * c * u;
+}
 
 }  // namespace f8blk
 

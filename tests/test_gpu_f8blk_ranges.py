@@ -53,6 +53,32 @@ def test_gated_unit_of_gates_down_to_where_the_exponential_overflows(pack, m, ff
     assert (off <= np.maximum(half_step(want), half_step(np.abs(want) + slack)) + slack)[whole].all()
 
 
+@pytest.mark.parametrize("m,ff,k,kernel", [(30, 128, 2048, 1), (40, 400, 2048, 1), (4000, 2064, 128, 2)])
+def test_gated_unit_of_gates_up_to_the_largest_f32(pack, m, ff, k, kernel):
+    """silu(g) is g for large gates, up to where f32 ends; the ups are small, so the result is an ordinary number."""
+    assert plan(pack, 2, m, ff, k)[0] == kernel
+    xq = torch.zeros(m, k, dtype=torch.uint8, device="cuda")
+    xq[:, 0] = ONE
+    g = torch.exp2(torch.linspace(120.0, 127.9, m, dtype=torch.float64, device="cuda")).float()           # a token's only scale, and its gate
+    gq, uq = torch.zeros(ff, k, dtype=torch.uint8, device="cuda"), torch.zeros(ff, k, dtype=torch.uint8, device="cuda")
+    gq[:, 0] = ONE
+    uq[:, 0] = (0x30 + torch.arange(ff, device="cuda") % 16).to(torch.uint8)
+    gs, us = torch.ones(blocks(ff), blocks(k), device="cuda"), torch.full((blocks(ff), blocks(k)), 2.0 ** -140, device="cuda")
+    hq, hs = torch.zeros(m * ff, dtype=torch.uint8, device="cuda"), torch.zeros(m * blocks(ff), device="cuda")
+    pack.call("pdk_f8blk_gate_up", gq, gs, uq, us, xq, g.view(m, 1).expand(m, blocks(k)).contiguous(), hq, hs, k, ff, m)
+    assert pack.device_error() == 0
+    g64 = g.double().cpu().numpy()[:, None]
+    h = g64 * (g64 * 2.0 ** -140 * e4m3_value(uq[:, 0].cpu().numpy())[None])
+    s = hs.cpu().numpy().reshape(m, -1).astype(np.float64)
+    rel = 12 * ULP                                                       # as above
+    amax = by_block(np.abs(h), 1).max(axis=(1, 3))
+    assert (np.abs(s * 448.0 - amax) <= (rel + 4 * ULP) * amax).all()
+    want = h / expand(s, 1, m, ff)
+    slack = (rel + 4 * ULP) * np.abs(want)
+    off = np.abs(e4m3_value(hq.cpu().numpy()).reshape(m, ff) - want)
+    assert (off <= np.maximum(half_step(want), half_step(np.abs(want) + slack)) + slack).all()
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 272, 2048), (40, 400, 2048), (4000, 2064, 384), (300, 700, 256)])
 @pytest.mark.parametrize("xs,ws", [(2.0 ** -60, 2.0 ** -66), (2.0 ** -126, 1.0), (2.0 ** 100, 2.0 ** 9), (2.0 ** -100, 2.0 ** 120)])
 def test_products_under_scales_whose_product_f32_holds(pack, m, n, k, xs, ws):
