@@ -9,7 +9,7 @@
 //               scale is the token's times the plane's; each warp keeps the BN products of a block in a row of shared memory of its own and
 //               reads them back as broadcasts.
 // The partial products meet through distributed shared memory and are added in rank order: the same bits whatever the timing.  A store
-// that may be past the batch is predicated, not branched around (60 tokens through a gated 2880 x 2880 front 14.0 -> 9.7 us with tiles of 32).
+// that may be past the batch is predicated, not branched around (60 tokens through a gated 2880 x 2880 front 14.0 -> 9.8 us with tiles of 32).
 // HBM bounds it: 1 token through 5120 x 17408 15.5 us, 5.7 TB/s; its gated front 28 us, 6.3 TB/s; 7 tokens through 17408 x 5003 16.2 us, 5.4 TB/s.  Below
 // some MB of weights it is start-up and meeting: 1 token through 5120 x 1024 4.5 us, of which the stream takes 0.8.
 // Gated front: gate and up of a channel are in one thread's registers.  They meet by token: the owner of a token has all 128
